@@ -152,6 +152,97 @@ int cmolhip_attn_decode(cmolhip_ctx_t *c, int n, const float *q,
                         const int32_t *seqlen, int n_heads, int n_kv,
                         int d_head, int max_ctx, int kv_f16, int split, float *out);
 
+/* ---- serving operators ---------------------------------------------------
+ * No reference counterpart (the reference decodes one session at a time over
+ * its whole context and picks tokens on the host).  Each call launches its
+ * kernels on the context's stream and returns without waiting for them; it
+ * allocates nothing, touches neither the arena nor any state of the library,
+ * and may be captured into a HIP graph.  Its scratch is `ws`, ws_bytes >= what
+ * the operator's _bytes function gives for the same arguments; the contents
+ * need not be kept or cleared, but calls that may run at the same time (other
+ * streams, graphs replayed beside each other) need a workspace each.  The
+ * _bytes functions need no device and give 0 for arguments that the call
+ * refuses.  Refusals (CMOL_ERR_ARGS, or CMOL_ERR_UNSUPPORTED for a d_head
+ * other than 16, 32, 64, 128 and 256) launch nothing.  Device pointers; q, out,
+ * ws and the caches 16-byte aligned.
+ *
+ * Caches hold fp32 or, with kv_f16, fp16 values.  Session i's cache starts at
+ * element slots[i] * slot_stride (slots: device int32, NULL: i; slot_stride 0:
+ * n_kv * max_ctx * d_head, else a multiple of 8 that is no smaller) and is
+ * [n_kv][max_ctx][d_head]; query head h reads kv head h / (n_heads / n_kv).
+ * seqlen[n] (device int32) is the number of positions in the cache, the
+ * token's own among them, taken as max_ctx where it is above.  Scores are
+ * q . k / sqrt(d_head); a row that sees no position (a length of 0 or below, a
+ * slot below 0: padding of a batch) is 0.  Positions a row does not see do not
+ * reach it whatever they hold.  Sums and softmax statistics are fp32. */
+
+/* Decode attention of n sessions (1..65535) over a sliding window with sinks:
+ * a session of length L sees positions t < sinks and t >= L - window (window
+ * >= 1 counts the token's own position; sinks >= 0).  q and out
+ * [n][n_heads * d_head]. */
+size_t cmolhip_attn_window_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window,
+                                 int sinks);
+int cmolhip_attn_window(cmolhip_ctx_t *c, int n, const float *q, const void *kcache,
+                        const void *vcache, const int32_t *slots, size_t slot_stride,
+                        const int32_t *seqlen, int n_heads, int n_kv, int d_head, int max_ctx,
+                        int kv_f16, int window, int sinks, void *ws, size_t ws_bytes, float *out);
+
+/* The same for n consecutive tokens (1..65535) of one session, whose cache
+ * kcache / vcache is: token i at position pos0 + i (pos0 + n <= max_ctx) sees
+ * t <= pos0 + i with t < sinks or t > pos0 + i - window. */
+size_t cmolhip_attn_window_prompt_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx,
+                                        int window, int sinks);
+int cmolhip_attn_window_prompt(cmolhip_ctx_t *c, int n, int pos0, const float *q,
+                               const void *kcache, const void *vcache, int n_heads, int n_kv,
+                               int d_head, int max_ctx, int kv_f16, int window, int sinks, void *ws,
+                               size_t ws_bytes, float *out);
+
+/* Decode attention of n sessions (1..65535) that share a prefix, cached once:
+ * every session sees the prefix_len (0..prefix_ctx) positions of kprefix /
+ * vprefix [n_kv][prefix_ctx][d_head] (an array of its own, or one slot's cache
+ * with prefix_ctx = max_ctx) and then its own seqlen[i] positions, which may
+ * be none (a slot below 0: the prefix alone). */
+size_t cmolhip_attn_shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len,
+                                 int max_ctx);
+int cmolhip_attn_shared(cmolhip_ctx_t *c, int n, const float *q, const void *kprefix,
+                        const void *vprefix, int prefix_len, int prefix_ctx, const void *kcache,
+                        const void *vcache, const int32_t *slots, size_t slot_stride,
+                        const int32_t *seqlen, int n_heads, int n_kv, int d_head, int max_ctx,
+                        int kv_f16, void *ws, size_t ws_bytes, float *out);
+
+/* From logits to the next token, n rows (1..65535) at once: penalties for
+ * repeated tokens, biases, grammar masks and the greedy choice.  For token v
+ * of row i, with c occurrences in the row's history:
+ *   x1 = c times: x > 0 ? x / repeat[i] : x * repeat[i]   (repeat[i] > 1; each
+ *        result rounded, as cmol_apply_repeat_penalty does)
+ *   x2 = x1 - (frequency[i] * c + presence[i])            (c > 0)
+ *   x3 = x2 + the bias of v
+ *   x4 = x3, or -inf where the row's mask does not allow v
+ * out receives x4; next[i] the lowest index of the row's largest x4, -1 where
+ * nothing above -inf is left (a NaN is never chosen).  All pointers device;
+ * those of parts that are not wanted are NULL. */
+typedef struct {
+    int32_t n, vocab;
+    int64_t stride;              /* elements between rows of logits and of out, >= vocab */
+    const float *logits;
+    float *out;                  /* may be logits itself; NULL: only the choice  */
+    int32_t *next;               /* [n]; NULL: no choice                         */
+    const int32_t *history;      /* [n][history_cap] token ids in any order (ids outside the vocabulary count for nothing) */
+    const int32_t *history_len;  /* [n], taken as 0..history_cap                 */
+    int32_t history_cap;
+    const float *repeat, *frequency, *presence;   /* [n] each                    */
+    const int32_t *bias_ids;     /* [n][bias_cap]; of an id listed twice the last entry counts */
+    const float *bias;           /* [n][bias_cap]                                */
+    const int32_t *bias_len;     /* [n], taken as 0..bias_cap                    */
+    int32_t bias_cap;
+    const uint32_t *mask;        /* [mask_rows][(vocab + 31) / 32]: bit v % 32 of word v / 32 set: v is allowed */
+    const int32_t *mask_row;     /* [n]: the mask row of each row, any other value none; NULL: row i has mask row i */
+    int32_t mask_rows;
+} cmolhip_logits_t;
+
+size_t cmolhip_logits_bytes(int n, int vocab);
+int cmolhip_logits(cmolhip_ctx_t *c, const cmolhip_logits_t *p, void *ws, size_t ws_bytes);
+
 /* ---- whole-model decode path ------------------------------------------- */
 typedef struct cmolhip_model cmolhip_model_t;
 

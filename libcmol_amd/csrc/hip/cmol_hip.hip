@@ -17,7 +17,9 @@
 
 #include "../../../include/cmol_hip.h"
 #include "common.h"
+#include "attn_rows.h"
 #include "kernels.h"
+#include "logits.h"
 
 namespace {
 
@@ -560,6 +562,212 @@ int cmolhip_attn_decode(cmolhip_ctx_t *c, int n, const float *q, const void *kca
     } while (0);
     arena_release(c, mark);
     return rc;
+}
+
+} // extern "C"
+
+// ---------------------------------------------------------------------------
+// Serving operators
+// ---------------------------------------------------------------------------
+namespace {
+
+// The context's device current for a call, the caller's again after it.
+struct OnDevice {
+    int prev = -1;
+    bool ok;
+    explicit OnDevice(int device)
+    {
+        ok = hipGetDevice(&prev) == hipSuccess;
+        if (ok && prev == device) prev = -1;
+        else if (ok) ok = hipSetDevice(device) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
+    }
+    ~OnDevice()
+    {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Shapes the rows kernels take: a workspace size, or 0 for a refusal (*rc).
+bool rows_shape(int n, int n_heads, int n_kv, int d_head, int max_ctx, int *rc)
+{
+    *rc = E_ARGS;
+    if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_kv > 65535 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
+    if (d_head < 1 || (size_t)n_heads * d_head > INT32_MAX) return false;
+    *rc = E_UNSUPPORTED;
+    if (d_head != 16 && d_head != 32 && d_head != 64 && d_head != 128 && d_head != 256) return false;
+    *rc = E_OK;
+    return true;
+}
+
+size_t window_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int *rc)
+{
+    if (!rows_shape(n, n_heads, n_kv, d_head, max_ctx, rc)) return 0;
+    if (window < 1 || sinks < 0) {
+        *rc = E_ARGS;
+        return 0;
+    }
+    return ALIGN;
+}
+
+size_t shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx, int *rc)
+{
+    if (!rows_shape(n, n_heads, n_kv, d_head, max_ctx, rc)) return 0;
+    if (prefix_len < 0) {
+        *rc = E_ARGS;
+        return 0;
+    }
+    return ALIGN;
+}
+
+// What the attention calls share: pointers and workspace checked, arguments
+// laid out (`need`: the workspace size, 0 a refusal already in *rc).
+bool rows_args(RowsArgs &a, cmolhip_ctx_t *c, int n, const float *q, const void *k, const void *v, const int32_t *slots,
+               size_t slot_stride, int n_heads, int n_kv, int d_head, int max_ctx, int kv_f16, const void *ws,
+               size_t ws_bytes, size_t need, float *out, int *rc)
+{
+    if (!need) return false;
+    *rc = E_ARGS;
+    const size_t packed = (size_t)n_kv * max_ctx * d_head;
+    if (!c || !q || !k || !v || !out || !ws || ws_bytes < need) return false;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(ws)) return false;
+    if (slot_stride && (slot_stride < packed || slot_stride % 8)) return false;
+    *rc = E_OK;
+    a.q = q;
+    a.out = out;
+    a.k = k;
+    a.v = v;
+    a.slots = slots;
+    a.slot_stride = slot_stride ? slot_stride : packed;
+    a.n = n;
+    a.n_heads = n_heads;
+    a.n_kv = n_kv;
+    a.d_head = d_head;
+    a.max_ctx = max_ctx;
+    a.kv_f16 = kv_f16 != 0;
+    return true;
+}
+
+} // namespace
+
+extern "C" {
+
+size_t cmolhip_attn_window_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
+{
+    int rc;
+    return window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
+}
+
+int cmolhip_attn_window(cmolhip_ctx_t *c, int n, const float *q, const void *kcache, const void *vcache,
+                        const int32_t *slots, size_t slot_stride, const int32_t *seqlen, int n_heads, int n_kv,
+                        int d_head, int max_ctx, int kv_f16, int window, int sinks, void *ws, size_t ws_bytes, float *out)
+{
+    int rc;
+    RowsArgs a{};
+    const size_t need = window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
+    if (!rows_args(a, c, n, q, kcache, vcache, slots, slot_stride, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes,
+                   need, out, &rc))
+        return rc;
+    if (!seqlen) return E_ARGS;
+    a.seqlen = seqlen;
+    a.window = std::min(window, max_ctx);
+    a.sinks = std::min(sinks, max_ctx);
+    OnDevice on(c->device);
+    return on.ok ? launch_attn_window(a, c->stream) : E_INVALID;
+}
+
+size_t cmolhip_attn_window_prompt_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
+{
+    int rc;
+    return n <= max_ctx ? window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc) : 0;
+}
+
+int cmolhip_attn_window_prompt(cmolhip_ctx_t *c, int n, int pos0, const float *q, const void *kcache, const void *vcache,
+                               int n_heads, int n_kv, int d_head, int max_ctx, int kv_f16, int window, int sinks,
+                               void *ws, size_t ws_bytes, float *out)
+{
+    int rc;
+    RowsArgs a{};
+    const size_t need = window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
+    if (need && (pos0 < 0 || n > max_ctx || pos0 > max_ctx - n)) return E_ARGS;
+    if (!rows_args(a, c, n, q, kcache, vcache, nullptr, 0, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes, need,
+                   out, &rc))
+        return rc;
+    a.pos0 = pos0;
+    a.window = std::min(window, max_ctx);
+    a.sinks = std::min(sinks, max_ctx);
+    OnDevice on(c->device);
+    return on.ok ? launch_attn_window(a, c->stream) : E_INVALID;
+}
+
+size_t cmolhip_attn_shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx)
+{
+    int rc;
+    return shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &rc);
+}
+
+int cmolhip_attn_shared(cmolhip_ctx_t *c, int n, const float *q, const void *kprefix, const void *vprefix,
+                        int prefix_len, int prefix_ctx, const void *kcache, const void *vcache, const int32_t *slots,
+                        size_t slot_stride, const int32_t *seqlen, int n_heads, int n_kv, int d_head, int max_ctx,
+                        int kv_f16, void *ws, size_t ws_bytes, float *out)
+{
+    int rc;
+    RowsArgs a{};
+    const size_t need = shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &rc);
+    if (!rows_args(a, c, n, q, kcache, vcache, slots, slot_stride, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes,
+                   need, out, &rc))
+        return rc;
+    if (!seqlen || prefix_len > prefix_ctx || (prefix_len && (!kprefix || !vprefix))) return E_ARGS;
+    if (!aligned16(kprefix) || !aligned16(vprefix)) return E_ARGS;
+    a.seqlen = seqlen;
+    a.pk = kprefix;
+    a.pv = vprefix;
+    a.prefix = prefix_len;
+    a.prefix_ctx = prefix_ctx;
+    a.window = max_ctx;
+    OnDevice on(c->device);
+    return on.ok ? launch_attn_shared(a, c->stream) : E_INVALID;
+}
+
+size_t cmolhip_logits_bytes(int n, int vocab)
+{
+    if (n < 1 || n > GEMM_MAX_N || vocab < 1) return 0;
+    return align_up((size_t)n * logits_slabs(vocab) * sizeof(unsigned long long), ALIGN);
+}
+
+int cmolhip_logits(cmolhip_ctx_t *c, const cmolhip_logits_t *p, void *ws, size_t ws_bytes)
+{
+    if (!c || !p || !ws || !aligned16(ws)) return E_ARGS;
+    const size_t need = cmolhip_logits_bytes(p->n, p->vocab);
+    if (!need || ws_bytes < need || p->stride < p->vocab || !p->logits || (!p->out && !p->next)) return E_ARGS;
+    if (p->history && (!p->history_len || p->history_cap < 0)) return E_ARGS;
+    if (p->bias_ids && (!p->bias || !p->bias_len || p->bias_cap < 0)) return E_ARGS;
+    if (p->mask && (p->mask_rows < 1 || (!p->mask_row && p->mask_rows < p->n))) return E_ARGS;
+    LogitsArgs a{};
+    a.n = p->n;
+    a.vocab = p->vocab;
+    a.stride = p->stride;
+    a.x = p->logits;
+    a.out = p->out;
+    a.next = p->next;
+    a.history = p->history;
+    a.history_len = p->history_len;
+    a.history_cap = p->history_cap;
+    a.repeat = p->repeat;
+    a.frequency = p->frequency;
+    a.presence = p->presence;
+    a.bias_ids = p->bias_ids;
+    a.bias = p->bias;
+    a.bias_len = p->bias_len;
+    a.bias_cap = p->bias_cap;
+    a.mask = p->mask;
+    a.mask_row = p->mask_row;
+    a.mask_rows = p->mask_rows;
+    a.part = (unsigned long long *)ws;
+    OnDevice on(c->device);
+    return on.ok ? launch_logits(a, c->stream) : E_INVALID;
 }
 
 } // extern "C"

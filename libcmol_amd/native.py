@@ -50,6 +50,15 @@ class QTensor(C.Structure):
                 ("row_tiles", I32), ("block_quads", I32), ("fold", I32)]
 
 
+class Logits(C.Structure):
+    """cmolhip_logits_t"""
+    _fields_ = [("n", I32), ("vocab", I32), ("stride", C.c_int64), ("logits", P), ("out", P), ("next", P),
+                ("history", P), ("history_len", P), ("history_cap", I32),
+                ("repeat", P), ("frequency", P), ("presence", P),
+                ("bias_ids", P), ("bias", P), ("bias_len", P), ("bias_cap", I32),
+                ("mask", P), ("mask_row", P), ("mask_rows", I32)]
+
+
 # (name, restype, argtypes) of every exported entry point declared in include/*.h
 SIGNATURES = [
     # cmol.h
@@ -95,6 +104,17 @@ SIGNATURES = [
     ("cmolhip_noalloc_scratch_bytes", C.c_size_t, []),
     ("cmolhip_attn_decode", C.c_int, [P, C.c_int, P, P, P, P, C.c_int, C.c_int, C.c_int,
                                       C.c_int, C.c_int, C.c_int, P]),
+    ("cmolhip_attn_window_bytes", C.c_size_t, [C.c_int] * 7),
+    ("cmolhip_attn_window", C.c_int, [P, C.c_int, P, P, P, P, C.c_size_t, P] + [C.c_int] * 7 +
+     [P, C.c_size_t, P]),
+    ("cmolhip_attn_window_prompt_bytes", C.c_size_t, [C.c_int] * 7),
+    ("cmolhip_attn_window_prompt", C.c_int, [P, C.c_int, C.c_int, P, P, P] + [C.c_int] * 7 +
+     [P, C.c_size_t, P]),
+    ("cmolhip_attn_shared_bytes", C.c_size_t, [C.c_int] * 6),
+    ("cmolhip_attn_shared", C.c_int, [P, C.c_int, P, P, P, C.c_int, C.c_int, P, P, P, C.c_size_t, P] +
+     [C.c_int] * 5 + [P, C.c_size_t, P]),
+    ("cmolhip_logits_bytes", C.c_size_t, [C.c_int, C.c_int]),
+    ("cmolhip_logits", C.c_int, [P, P, P, C.c_size_t]),
     ("cmolhip_model_plan", C.c_int, [P, C.POINTER(C.c_size_t)]),
     ("cmolhip_gemv_scratch_floats", C.c_size_t, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
     ("cmolhip_batch_scratch_floats", C.c_int, [P, C.c_int, C.POINTER(C.c_size_t)]),
