@@ -7,8 +7,39 @@
 //   shared   the prefix's positions, then its own t < seqlen
 // and out = sum_t softmax_t(q . k_t / sqrt(d_head)) v_t over them, 0 where
 // there are none.  Every sum and softmax statistic is fp32.
+//
+// One walk serves all of them (rows_walk): a wave holds RT tiles of 16 query
+// rows of one kv head and takes tiles of 32 cached positions, straight from
+// the cache into the matrix instructions' operand registers; nothing is staged
+// in LDS and the waves of a work-group, on different tiles, meet only at the
+// end of their range (rows_finish).
+//   * scores transposed, S^T = K Q^T: the A operand's rows are 16 positions
+//     (16-byte pieces of the K rows as cached), the B operand's columns the
+//     query rows, so lane (col, g) holds positions 4g .. 4g+3 of row `col`;
+//   * O^T += V^T P^T: the scores' layout is the B operand's as it is (k index
+//     of lane group g = positions 4g .. 4g+3, and 16 more of the tile's second
+//     half), and a lane's A operand for output tile e is dimension VD col + e of
+//     those positions, VD = d_head / 16: a lane loads VD neighbouring dimensions
+//     of its positions' V rows, 16 lanes a whole row, and for fp16 pairs of rows
+//     are interleaved with one v_perm_b32 per two values;
+//   * online softmax whose reference moves only when a score exceeds it by more
+//     than RW_LAZY (log2 units; a wave vote), so most tiles need no cross-lane
+//     step; weights are 2^(t c2 + mk), c2 = log2(e) / sqrt(d_head).
+// fp16 caches: 16x16x32 f16 products, exact, with fp32 sums.  The query is
+// scaled by a power of two per row into [1, 2) and split into two f16 parts (22
+// bits); a weight, scaled by 2^RW_SCALE, into two f16 parts whose products
+// share an accumulator (22 bits of a weight down to 2^-16 of the largest, an
+// absolute 2^-36 of it below).  fp32 caches: 16x16x4 f32 products throughout.
 #pragma once
 #include "common.h"
+
+#include <algorithm>
+
+constexpr int RW_TP = 32;            // positions per tile
+constexpr int RW_NW = 4;             // waves per work-group
+constexpr int RW_PAD = 2;            // tiles that stand for the start of an item's piece
+constexpr float RW_LAZY = 2.0f;      // log2: weights stay below 2^(RW_SCALE + 2)
+constexpr float RW_SCALE = 12.0f;
 
 struct RowsArgs {
     const float *q;            // [n][n_heads*d_head]
@@ -22,27 +53,471 @@ struct RowsArgs {
     int pos0;                  // prompt: position of item 0 (seqlen null)
     const void *pk, *pv;       // shared prefix [n_kv][prefix_ctx][d_head]
     int prefix, prefix_ctx;
+    // work split (rows_plan_*) and its partial results: (m, l, o[d_head]) per
+    // query row and part; a weight sum is l 2^m
+    int bal;                   // balanced ranges of the items' own positions (0: one work-group per item)
+    int parts;                 // parts of the prefix, or of a prompt block's positions
+    float *pm, *pl, *po;       // [n_kv][bal + n][G]
+    float *xm, *xl, *xo;       // [n_kv][n * G][parts]
 };
+
+// ---- which positions -----------------------------------------------------------
+
+// Tiles of two runs of positions, [0, s) and [lo, hi): the first ns tiles
+// cover the first, the rest the second.
+struct RowsLine {
+    int s, lo, hi, ns;
+    __device__ __forceinline__ int tiles() const { return ns + (hi - lo + RW_TP - 1) / RW_TP; }
+    // first position and number of positions of tile u
+    __device__ __forceinline__ void tile(int u, int *p0, int *cnt) const
+    {
+        *p0 = u < ns ? u * RW_TP : lo + (u - ns) * RW_TP;
+        *cnt = min(RW_TP, (u < ns ? s : hi) - *p0);
+    }
+};
+
+// Positions that tokens at first .. last see between them.
+__device__ __forceinline__ RowsLine rows_line(int first, int last, int window, int sinks)
+{
+    RowsLine l;
+    l.hi = last + 1;
+    l.lo = max(first + 1 - window, 0);
+    l.s = min(sinks, l.lo);
+    l.ns = (l.s + RW_TP - 1) / RW_TP;
+    return l;
+}
 
 // Positions of item i's cache up to its own (0: it sees nothing there), and
 // that cache.
 __device__ __forceinline__ int rows_item(const RowsArgs &a, int i, size_t *base)
 {
-    if (!a.seqlen) {
-        *base = 0;
-        return a.pos0 + i + 1;
-    }
     const int slot = a.slots ? a.slots[i] : i;
+    const int L = a.seqlen[i];
     *base = slot < 0 ? 0 : (size_t)slot * a.slot_stride;
-    return slot < 0 ? 0 : max(min(a.seqlen[i], a.max_ctx), 0);
+    return slot < 0 ? 0 : max(min(L, a.max_ctx), 0);
 }
 
-// One query row on one wave: lane l holds dimensions DL l .. +DL-1 (the first
-// d_head lanes below 64).
+__device__ __forceinline__ unsigned rows_tiles(const RowsArgs &a, int i)
+{
+    if (i >= a.n) return 0;
+    size_t base;
+    const int L = rows_item(a, i, &base);
+    return L > 0 ? rows_line(L - 1, L - 1, a.window, a.sinks).tiles() : 0;
+}
+
+// Balanced ranges.  The items' tiles are laid end to end on one line, each
+// item preceded by RW_PAD tiles for the fixed cost of starting a piece; range
+// w holds the line's tiles [w R, w R + R).  The cut of item i in range w is a
+// piece, in slot w + i (unique: pieces are in line order), so an item's pieces
+// are consecutive slots and every work-group of `bal + n` finds its own piece,
+// if any, from the lengths alone.
+__device__ __forceinline__ unsigned wave_sum_u(unsigned v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ unsigned wave_scan_u(unsigned v)   // inclusive
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned t = __shfl_up(v, o, 64);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+constexpr unsigned RW_RMIN = 4;   // tiles per range at least: one per wave
+
+// Range length; t0: this lane's item's tiles among the first 64.
+__device__ __forceinline__ unsigned rows_range(const RowsArgs &a, unsigned t0)
+{
+    const int lane = threadIdx.x & 63;
+    unsigned t = lane < a.n ? t0 + RW_PAD : 0;
+    for (int b = 64; b < a.n; b += 64) t += b + lane < a.n ? rows_tiles(a, b + lane) + RW_PAD : 0;
+    const unsigned line = wave_sum_u(t);
+    return max(RW_RMIN, (line + a.bal - 1) / a.bal);
+}
+
+// The piece of slot k: its item (-1: none) and the item's tiles [u0, u1);
+// whole: the item's only one.
+__device__ __forceinline__ int rows_piece(const RowsArgs &a, int k, int *u0, int *u1, bool *whole)
+{
+    const int lane = threadIdx.x & 63;
+    const unsigned t0 = rows_tiles(a, lane);
+    const unsigned R = rows_range(a, t0);
+    unsigned base = 0;
+    for (int b = 0; b < a.n; b += 64) {
+        const unsigned T = b == 0 ? t0 : rows_tiles(a, b + lane);
+        const unsigned v = b + lane < a.n ? T + RW_PAD : 0, inc = wave_scan_u(v);
+        const unsigned at = base + inc - v + RW_PAD;   // the item's first tile on the line
+        const int w = k - (b + lane);
+        const uint64_t m = __ballot(T > 0 && w >= (int)(at / R) && w <= (int)((at + T - 1) / R));
+        if (m) {
+            const int j = __builtin_ctzll(m), i = b + j;
+            const int n = __builtin_amdgcn_readlane(T, j);
+            const int r0 = (int)((unsigned)(k - i) * R - (unsigned)__builtin_amdgcn_readlane(at, j));
+            *u0 = max(r0, 0);
+            *u1 = min(r0 + (int)R, n);
+            *whole = r0 <= 0 && r0 + (int)R >= n;
+            return i;
+        }
+        base += __builtin_amdgcn_readlane(inc, 63);
+    }
+    return -1;
+}
+
+// The slots of item i's pieces: the first, and how many.
+__device__ __forceinline__ int rows_pieces(const RowsArgs &a, int i, int *first)
+{
+    const int lane = threadIdx.x & 63;
+    const unsigned t0 = rows_tiles(a, lane), R = rows_range(a, t0);
+    unsigned pre = 0;
+    for (int b = 0; b < i; b += 64) pre += b + lane < i ? (b == 0 ? t0 : rows_tiles(a, b + lane)) + RW_PAD : 0;
+    const unsigned at = wave_sum_u(pre) + RW_PAD, T = rows_tiles(a, i);
+    *first = (int)(at / R) + i;
+    return T ? (int)((at + T - 1) / R - at / R) + 1 : 0;
+}
+
+// ---- the walk ------------------------------------------------------------------
+
+// A wave's query rows and their online softmaxes: lane (col, g) = (lane % 16,
+// lane / 16) holds row 16 rt + col of tile rt.
+template <int DH, typename KT, int RT>
+struct RowsWave {
+    static constexpr bool F16 = sizeof(KT) == 2;
+    static constexpr int VD = DH / 16;               // dimensions per lane of a V row, output tiles
+    static constexpr int KS = DH < 32 ? 1 : DH / 32; // f16 k-steps of a score
+    f16x8 qh[RT][F16 ? KS : 1], ql[RT][F16 ? KS : 1];
+    f32x4 qf[RT][F16 ? 1 : VD];
+    float c2[RT];            // log2 units per raw score
+    f32x4 o[RT][VD];         // o[rt][e][i]: dimension VD (4g + i) + e of the row
+    float m[RT], mk[RT], l[RT];   // l: this lane's positions only
+
+    // row r's query at q(r)
+    template <typename Q>
+    __device__ __forceinline__ void start(Q q)
+    {
+#pragma clang fp contract(off)
+        const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+        const float sc = 1.44269504088896341f / sqrtf((float)DH);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            const float *p = q(16 * rt + col);
+            c2[rt] = sc;
+            if constexpr (F16) {
+                float x[KS][8], top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const float4 a = ldg((const float4 *)(p + (32 * s + 8 * g) % DH));
+                    const float4 b = ldg((const float4 *)(p + (32 * s + 8 * g) % DH + 4));
+                    const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[s][e] = DH < 32 && g >= 2 ? 0.0f : y[e];   // (d_head 16: half a k-step)
+                        top = fmaxf(top, fabsf(x[s][e]));
+                    }
+                }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                // the largest into [1, 2) (below 2^-100 less, so that c2 stays
+                // above 0); a row of zeros, infinities or NaN as it is
+                const int ex = top > 0.0f && top < INFINITY ? max(ilogbf(top), -100) : 0;
+                c2[rt] = ldexpf(sc, ex);
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = ldexpf(x[s][e], -ex);
+                        const _Float16 hi = (_Float16)y;
+                        qh[rt][s][e] = hi;
+                        ql[rt][s][e] = (_Float16)((y - (float)hi) * 2048.0f);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VD; i++) qf[rt][i] = ldg((const f32x4 *)(p + 16 * i + 4 * g));
+            }
+            m[rt] = -INFINITY;
+            mk[rt] = RW_SCALE;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int e = 0; e < VD; e++) o[rt][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+};
+
+// Mask of the rows of a prompt block: row r's token is at position pos[rt].
+struct RowsSeen {
+    int first, last, window, sinks;   // positions of the block's tokens
+    const int *pos;
+};
+
+// Tiles u, u + step, .. below u1 of `line` into the wave's rows, K and V rows
+// of the kv head at kb and vb.  MASKED: rows see different positions (seen).
+template <int DH, typename KT, int RT, bool MASKED>
+__device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb, const KT *vb, const RowsLine &line, int u,
+                                          int u1, int step, const RowsSeen *seen)
+{
+#pragma clang fp contract(off)
+    typedef RowsWave<DH, KT, RT> W;
+    constexpr bool F16 = W::F16;
+    constexpr int VD = W::VD, KS = W::KS, ES = sizeof(KT);
+    constexpr int VB = VD * ES;                        // bytes of a lane's piece of a V row
+    constexpr int VW = VB < 4 ? 1 : VB / 4;            // dwords of it
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    if (u >= u1) return;
+    const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    f16x8 kh[F16 ? 2 : 1][F16 ? KS : 1];
+    f32x4 kf[F16 ? 1 : 2][F16 ? 1 : VD];
+    uint32_t vr[8][VW];                                // rows 4g + r (r < 4), 16 + 4g + r - 4
+    auto load_k = [&](int t) {
+        int p0, cnt;
+        line.tile(t, &p0, &cnt);
+        const char *base = (const char *)uniform_ptr(kb + (size_t)p0 * DH);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const unsigned at = (unsigned)min(16 * c + col, cnt - 1) * (DH * ES);
+            if constexpr (F16) {
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    kh[c][s] = ldg((const f16x8 *)(base + (at + (64 * s + 16 * g) % (DH * ES))));
+                    if (DH < 32 && g >= 2) kh[c][s] = f16x8{};
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VD; i++) kf[c][i] = ldg((const f32x4 *)(base + (at + 64 * i + 16 * g)));
+            }
+        }
+    };
+    auto load_v = [&](int t) {
+        int p0, cnt;
+        line.tile(t, &p0, &cnt);
+        const char *base = (const char *)uniform_ptr(vb + (size_t)p0 * DH);
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            const int row = (r < 4 ? 0 : 12) + 4 * g + r;
+            const char *src = base + ((unsigned)min(row, cnt - 1) * (DH * ES) + VB * col);
+            if constexpr (VB == 2) vr[r][0] = *gptr((const uint16_t *)src);
+            else if constexpr (VB == 4) vr[r][0] = ldg((const uint32_t *)src);
+            else if constexpr (VB == 8) {
+                const u32x2 x = ldg((const u32x2 *)src);
+                vr[r][0] = x[0];
+                vr[r][1] = x[1];
+            } else {
+#pragma unroll
+                for (int b = 0; b < VB / 16; b++) {
+                    const u32x4 x = ldg((const u32x4 *)(src + 16 * b));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) vr[r][4 * b + e] = x[e];
+                }
+            }
+        }
+    };
+    load_k(u);
+    load_v(u);
+    for (; u < u1; u += step) {
+        int p0, cnt;
+        line.tile(u, &p0, &cnt);
+        // ---- scores: sc[rt][c][i] = position p0 + 16c + 4g + i of row 16 rt + col
+        float sc[RT][2][4];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                f32x4 s1 = zero4;
+                if constexpr (F16) {
+                    f32x4 s2 = zero4;
+#pragma unroll
+                    for (int s = 0; s < KS; s++) {
+                        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.qh[rt][s], s1, 0, 0, 0);
+                        s2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.ql[rt][s], s2, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[rt][c][i] = fmaf(s2[i], 1.0f / 2048.0f, s1[i]);
+                } else {
+#pragma unroll
+                    for (int d = 0; d < VD; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][d][e], w.qf[rt][d][e], s1, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) sc[rt][c][i] = s1[i];
+                }
+            }
+        }
+        if (u + step < u1) load_k(u + step);
+        // ---- masks (uniform branches): the run's end; rows that see less
+        bool edge = cnt < RW_TP;
+        if constexpr (MASKED)
+            edge |= p0 + cnt - 1 > seen->first || (p0 + cnt - 1 >= seen->sinks && p0 <= seen->last - seen->window);
+        if (edge) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at = 16 * c + 4 * g + i, p = p0 + at;
+                        bool see = at < cnt;
+                        if constexpr (MASKED)
+                            see = see && p <= seen->pos[rt] && (p < seen->sinks || p > seen->pos[rt] - seen->window);
+                        if (!see) sc[rt][c][i] = -INFINITY;
+                    }
+        }
+        // V rows past the run: 0, not a copy of its last (0 weight times infinity)
+        if (cnt < RW_TP) {
+#pragma unroll
+            for (int r = 0; r < 8; r++)
+                if ((r < 4 ? 0 : 12) + 4 * g + r >= cnt) {
+#pragma unroll
+                    for (int e = 0; e < VW; e++) vr[r][e] = 0;
+                }
+        }
+        // ---- online softmax
+        f16x8 ph[F16 ? RT : 1], pl[F16 ? RT : 1];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float mx = sc[rt][0][0];
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[rt][c][i]);
+            if (__ballot((mx - w.m[rt]) * w.c2[rt] > RW_LAZY)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(w.m[rt], mx);
+                const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn * w.c2[rt];
+                const float al = w.m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - w.mk[rt]);
+                w.m[rt] = mn;
+                w.mk[rt] = mkn;
+                w.l[rt] *= al;
+#pragma unroll
+                for (int e = 0; e < VD; e++) w.o[rt][e] *= al;
+            }
+            float ls = 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], w.c2[rt], w.mk[rt]));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], w.c2[rt], w.mk[rt]));
+                    ls += e0 + e1;
+                    if constexpr (F16) {
+                        const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0, e1));
+                        const f16x2 lo = __builtin_bit_cast(
+                            f16x2, __builtin_amdgcn_cvt_pkrtz(e0 - (float)hi[0], e1 - (float)hi[1]));
+                        ph[rt][4 * c + i] = hi[0];
+                        ph[rt][4 * c + i + 1] = hi[1];
+                        pl[rt][4 * c + i] = lo[0];
+                        pl[rt][4 * c + i + 1] = lo[1];
+                    } else {
+                        sc[rt][c][i] = e0;
+                        sc[rt][c][i + 1] = e1;
+                    }
+                }
+            w.l[rt] += ls;
+        }
+        // ---- O^T += V^T P^T
+#pragma unroll
+        for (int e = 0; e < VD; e++) {
+            if constexpr (F16) {
+                u32x4 x;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    x[j] = __builtin_amdgcn_perm(vr[2 * j + 1][e / 2], vr[2 * j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+                const f16x8 va = __builtin_bit_cast(f16x8, x);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) {
+                    w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[rt], w.o[rt][e], 0, 0, 0);
+                    w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[rt], w.o[rt][e], 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++)
+                            w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * c + j][e]), sc[rt][c][j],
+                                                                              w.o[rt][e], 0, 0, 0);
+            }
+        }
+        if (u + step < u1) load_v(u + step);
+    }
+}
+
+// The waves of a work-group meet: put(r, m, l, d, x) gets, for every row r of
+// the work-group's 16 RT, the rows' sums over the waves: weight sum l 2^m and
+// the unnormalised output's dimensions d .. d+N-1 (x), from one thread each.
+template <int DH>
+struct RowsMeet {
+    static constexpr int DC = DH < 128 ? DH : 128;   // dimensions per round
+    __attribute__((aligned(16))) float o[RW_NW][16][DC + 4];
+    float m[RW_NW][16], l[RW_NW][16];
+};
+template <int DH, typename KT, int RT, typename P>
+__device__ __forceinline__ void rows_finish(RowsWave<DH, KT, RT> &w, RowsMeet<DH> &meet, P put)
+{
+    constexpr int VD = DH / 16, DC = RowsMeet<DH>::DC, N = DC / 16;   // dimensions per thread and round
+    auto &xo = meet.o;
+    auto &xm = meet.m, &xl = meet.l;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, col = lane & 15, g = lane >> 4;
+    const int r = tid >> 4, a = tid & 15;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        float l = w.l[rt];
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        // a lane's dimensions VD (4g + i) .. +VD-1 of round c: those in [c DC, c DC + DC)
+#pragma unroll
+        for (int c = 0; c < DH / DC; c++) {
+            if (rt || c) __syncthreads();
+            if (g == 0 && c == 0) {
+                xm[wid][col] = w.m[rt] == -INFINITY ? -INFINITY : -w.mk[rt];
+                xl[wid][col] = l;
+            }
+            if (VD * 4 * g / DC == c) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int e = 0; e < VD; e++) xo[wid][col][VD * (4 * g + i) - c * DC + e] = w.o[rt][e][i];
+            }
+            __syncthreads();
+            float mx = xm[0][r];
+#pragma unroll
+            for (int k = 1; k < RW_NW; k++) mx = fmaxf(mx, xm[k][r]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            float lt = 0.0f, x[N] = {};
+#pragma unroll
+            for (int k = 0; k < RW_NW; k++) {
+                const float f = __builtin_amdgcn_exp2f(xm[k][r] - ref);
+                lt += xl[k][r] * f;
+#pragma unroll
+                for (int e = 0; e < N; e++) x[e] += xo[k][r][N * a + e] * f;
+            }
+            put(16 * rt + r, mx, lt, c * DC + N * a, x);
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ void rows_store(float *p, const float (&x)[N])
+{
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) *(f32x4 *)(p + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) p[e] = x[e];
+    }
+}
+
+// ---- one row on one wave ---------------------------------------------------------
+// Lane l holds dimensions DL l .. +DL-1 (the first d_head lanes below 64).
 template <int DH>
 struct RowState {
     static constexpr int DL = DH < 64 ? 1 : DH / 64;
-    float q[DL], o[DL], m, l;
+    float q[DL], o[DL], m, l;   // m in log2 units
 };
 
 // Positions t0 .. t1-1 of the cache rows at k and v into a row's online
@@ -54,14 +529,15 @@ __device__ void row_walk(RowState<DH> &r, const KT *k, const KT *v, int t0, int 
     constexpr int DL = RowState<DH>::DL;
     const int lane = threadIdx.x & 63;
     const bool on = lane * DL < DH;
+    const float sc = 1.44269504088896341f / sqrtf((float)DH);
     for (int t = t0; t < t1; t++) {
         const size_t at = (size_t)t * DH + (on ? lane * DL : 0);
         float s = 0.0f;
 #pragma unroll
         for (int d = 0; d < DL; d++) s = fmaf(r.q[d], (float)k[at + d], s);
-        s = wave_sum(on ? s : 0.0f) * (1.0f / sqrtf((float)DH));
+        s = wave_sum(on ? s : 0.0f) * sc;
         const float mn = fmaxf(r.m, s), ref = mn == -INFINITY ? 0.0f : mn;
-        const float al = expf(r.m - ref), e = expf(s - ref);
+        const float al = exp2f(r.m - ref), e = exp2f(s - ref);
         r.m = s != s ? s : mn;   // (fmaxf drops a NaN)
         r.l = r.l * al + e;
 #pragma unroll
@@ -69,5 +545,100 @@ __device__ void row_walk(RowState<DH> &r, const KT *k, const KT *v, int t0, int 
     }
 }
 
+// ---- partial results -------------------------------------------------------------
+
+// The sum of a row's partial results by the LPR SG threads (d4, sg) of it, SG
+// groups taking every SG-th; at(j): where the j-th of np is.  Group 0's
+// threads get the finished dimensions 4 d4 .. +3 (np 0: zeros).
+template <int DH, int SG, typename F>
+__device__ __forceinline__ f32x4 rows_sum(int np, int d4, int sg, F at)
+{
+#pragma clang fp contract(off)
+    constexpr int U = 4;
+    float mx = -INFINITY, L = 0.0f;
+    f32x4 acc = {};
+    for (int j0 = sg; j0 < np; j0 += U * SG) {
+        float pm[U], pl[U];
+        f32x4 po[U];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const float *m, *l, *o;
+            at(min(j0 + i * SG, np - 1), &m, &l, &o);
+            pm[i] = j0 + i * SG < np ? *m : -INFINITY;
+            pl[i] = *l;
+            po[i] = *(const f32x4 *)(o + 4 * d4);
+        }
+        float mn = mx;
+#pragma unroll
+        for (int i = 0; i < U; i++) mn = fmaxf(mn, pm[i]);
+        const float ref = mn == -INFINITY ? 0.0f : mn, f = __builtin_amdgcn_exp2f(mx - ref);
+        mx = mn;
+        L *= f;
+        acc *= f;
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            if (j0 + i * SG >= np) break;   // (a repeated one may hold what is not finite)
+            const float e = __builtin_amdgcn_exp2f(pm[i] - ref);
+            L += pl[i] * e;
+            acc += po[i] * e;
+        }
+    }
+    if constexpr (SG > 1) {
+        constexpr int LPR = DH / 4;
+        __shared__ __attribute__((aligned(16))) f32x4 so[SG][LPR];
+        __shared__ float sm[SG], sl[SG];
+        so[sg][d4] = acc;
+        if (d4 == 0) {
+            sm[sg] = mx;
+            sl[sg] = L;
+        }
+        __syncthreads();
+        if (sg) return acc;
+        float M = sm[0];
+        for (int k = 1; k < SG; k++) M = fmaxf(M, sm[k]);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        L = 0.0f;
+        acc = f32x4{};
+        for (int k = 0; k < SG; k++) {
+            const float f = __builtin_amdgcn_exp2f(sm[k] - ref);
+            L += sl[k] * f;
+            acc += so[k][d4] * f;
+        }
+    }
+    return np ? acc / L : f32x4{};
+}
+
+// ---- work split ------------------------------------------------------------------
+
+constexpr int RW_WGS = 512;   // work-groups of a call to aim for: two per CU
+
+inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
+
+// Balanced ranges for n items of up to `span` tiles on `heads` work-groups
+// each: 0 (an item whole) where an item has at most two rounds of tiles for its
+// waves or the items alone fill the chip.
+int rows_plan_bal(int n, long heads, long span);
+
+// What a call of these shapes splits into, and the number of its partial
+// results.
+struct RowsPlan {
+    int bal = 0, parts = 0;
+    size_t pieces = 0, cross = 0;   // pm / pl / po, and xm / xl / xo
+};
+RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks);
+RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks);
+RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx);
+
 int launch_attn_window(const RowsArgs &a, hipStream_t s);
+int launch_attn_window_prompt(const RowsArgs &a, hipStream_t s);
 int launch_attn_shared(const RowsArgs &a, hipStream_t s);
+
+#define RW_BY_D_HEAD(d, F)          \
+    switch (d) {                    \
+    case 16: F(16) break;           \
+    case 32: F(32) break;           \
+    case 64: F(64) break;           \
+    case 128: F(128) break;         \
+    case 256: F(256) break;         \
+    default: return -4;             \
+    }

@@ -1,0 +1,170 @@
+// attn_shared.hip — decode attention of sessions that share a prefix
+// (attn_rows.h).  The prefix is read once for all of them: per kv head the
+// sessions' query rows (n G of them, session-major) form tiles of 16 that walk
+// the prefix's positions together, RT tiles per work-group and the positions in
+// `parts`; the sessions' own positions are walked as single tokens are, in
+// balanced ranges.  Both kinds of work-group are one launch, and the merge
+// takes the parts and the pieces of a row.
+#include "attn_rows.h"
+
+// work-groups of the prefix: (kv head, part) fastest, padded to the eight XCDs,
+// so the row blocks that read the same positions run on one XCD and its L2
+__host__ __device__ inline unsigned shared_lanes(const RowsArgs &a) { return (unsigned)(a.n_kv * a.parts + 7) / 8 * 8; }
+__host__ __device__ inline unsigned shared_prefix_wgs(const RowsArgs &a, int rt)
+{
+    const int rows = a.n * (a.n_heads / a.n_kv);
+    return a.prefix ? shared_lanes(a) * (unsigned)((rows + 16 * rt - 1) / (16 * rt)) : 0;
+}
+
+template <int DH, typename KT, int RT>
+__device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH> &meet, unsigned wg)
+{
+#pragma clang fp contract(off)
+    const int G = a.n_heads / a.n_kv, rows = a.n * G;
+    const unsigned lanes = shared_lanes(a), lane = wg % lanes;
+    const int kvh = lane / a.parts, part = lane % a.parts, r0 = wg / lanes * 16 * RT;
+    if (kvh >= a.n_kv) return;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    RowsLine line;
+    line.s = line.lo = line.ns = 0;
+    line.hi = a.prefix;
+    const int T = line.tiles(), R = (T + a.parts - 1) / a.parts;
+    const int u0 = min(part * R, T), u1 = min(u0 + R, T);
+    RowsWave<DH, KT, RT> w;
+    w.start([&](int r) {
+        r = min(r0 + r, rows - 1);
+        return a.q + ((size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G) * DH;
+    });
+    const size_t base = (size_t)kvh * a.prefix_ctx * DH;
+    rows_walk<DH, KT, RT, false>(w, (const KT *)a.pk + base, (const KT *)a.pv + base, line, u0 + wid, u1, RW_NW, nullptr);
+    const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;
+    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+        if (r0 + r >= rows) return;
+        const size_t at = x0 + (size_t)r * a.parts;
+        rows_store(a.xo + at * DH + d, x);
+        if (d == 0) {
+            a.xm[at] = m;
+            a.xl[at] = l;
+        }
+    });
+}
+
+template <int DH, typename KT>
+__device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH> &meet, unsigned wg)
+{
+#pragma clang fp contract(off)
+    const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
+    const int slot = wg / (a.n_kv * blocks), hb = wg % (a.n_kv * blocks), kvh = hb / blocks, r0 = hb % blocks * 16;
+    const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int i = slot, u0 = 0, u1 = 0;
+    bool whole;
+    if (a.bal) {
+        i = rows_piece(a, slot, &u0, &u1, &whole);
+        if (i < 0) return;
+    }
+    size_t base;
+    const int L = rows_item(a, i, &base);
+    if (L <= 0) return;
+    const RowsLine line = rows_line(L - 1, L - 1, a.window, a.sinks);
+    if (!a.bal) u1 = line.tiles();
+    const size_t row0 = (size_t)i * a.n_heads + (size_t)kvh * G;
+    RowsWave<DH, KT, 1> w;
+    w.start([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
+    base += (size_t)kvh * a.max_ctx * DH;
+    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, u0 + wid, u1, RW_NW, nullptr);
+    const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
+    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+        r += r0;
+        if (r >= G) return;
+        rows_store(a.po + (part + r) * DH + d, x);
+        if (d == 0) {
+            a.pm[part + r] = m;
+            a.pl[part + r] = l;
+        }
+    });
+}
+
+template <int DH, typename KT, int RT>
+__global__ __launch_bounds__(256) void k_shared(RowsArgs a)
+{
+    __shared__ RowsMeet<DH> meet;
+    const unsigned pre = shared_prefix_wgs(a, RT);
+    if (blockIdx.x < pre) shared_prefix<DH, KT, RT>(a, meet, blockIdx.x);
+    else shared_own<DH, KT>(a, meet, blockIdx.x - pre);
+}
+
+template <int DH>
+__global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
+{
+    constexpr int LPR = DH / 4;
+    const int G = a.n_heads / a.n_kv, h = blockIdx.x, kvh = h / G, i = blockIdx.y, tid = threadIdx.x;
+    const int pre = a.prefix ? a.parts : 0;
+    int first = i, np;
+    if (a.bal) np = rows_pieces(a, i, &first);
+    else {
+        size_t base;
+        np = rows_item(a, i, &base) > 0 ? 1 : 0;
+    }
+    const size_t x0 = ((size_t)kvh * a.n * G + (size_t)i * G + h % G) * a.parts;
+    const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
+    const f32x4 o = rows_sum<DH, 256 / LPR>(
+        pre + np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
+            const bool own = j >= pre;
+            const size_t at = own ? p0 + (size_t)(j - pre) * G : x0 + j;
+            *m = (own ? a.pm : a.xm) + at;
+            *l = (own ? a.pl : a.xl) + at;
+            *x = (own ? a.po : a.xo) + at * DH;
+        });
+    if (tid < LPR) *(f32x4 *)(a.out + ((size_t)i * a.n_heads + h) * DH + 4 * tid) = o;
+}
+
+// Row tiles of a prefix work-group: as many as the registers hold, no more than
+// there are rows.
+static int shared_rt(int n, int G, int d_head, int kv_f16)
+{
+    const long rows = (long)n * G;
+    return std::min(rows <= 16 ? 1 : rows <= 32 ? 2 : 4, d_head == 256 ? 1 : kv_f16 && d_head < 128 ? 4 : 2);
+}
+
+static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt)
+{
+    const long blocks = (long)n_kv * ceil_div((long)n * (n_heads / n_kv), 16 * rt);
+    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_TP), RW_NW)));
+}
+
+RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
+{
+    RowsPlan p;
+    const int G = n_heads / n_kv;
+    p.parts = 1;
+    for (int f16 = 0; f16 < 2; f16++)
+        p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16)));
+    p.cross = prefix ? (size_t)n * n_heads * p.parts : 0;
+    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_TP));
+    p.pieces = (size_t)n_kv * (p.bal + n) * G;
+    return p;
+}
+
+int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
+{
+    RowsArgs a = a0;
+    const int G = a.n_heads / a.n_kv, rt = shared_rt(a.n, G, a.d_head, a.kv_f16);
+    a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt));
+    const size_t wgs = shared_prefix_wgs(a, rt) + (size_t)a.n_kv * ceil_div(G, 16) * (a.bal + a.n);
+    if (wgs > INT32_MAX) return -6;
+    const dim3 grid((unsigned)wgs), block(256);
+#define LAUNCH(DH, KT, RT) hipLaunchKernelGGL((k_shared<DH, KT, RT>), grid, block, 0, s, a)
+#define SHA(DH)                                                                               \
+    if (rt == 1) { if (a.kv_f16) LAUNCH(DH, _Float16, 1); else LAUNCH(DH, float, 1); }        \
+    else if constexpr (DH < 256) {                                                            \
+        if (a.kv_f16) { if (rt == 2) LAUNCH(DH, _Float16, 2); else LAUNCH(DH, _Float16, 4); } \
+        else LAUNCH(DH, float, 2);                                                            \
+    }
+    RW_BY_D_HEAD(a.d_head, SHA)
+#undef SHA
+#undef LAUNCH
+#define MERGE(DH) hipLaunchKernelGGL(k_shared_merge<DH>, dim3(a.n_heads, a.n), block, 0, s, a);
+    RW_BY_D_HEAD(a.d_head, MERGE)
+#undef MERGE
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}

@@ -1,64 +1,272 @@
-// attn_window.hip — attention over a sliding window with sinks, one wave per
-// (query head, item).
+// attn_window.hip — attention over a sliding window with sinks (attn_rows.h):
+// single tokens of many sessions, and consecutive tokens of one.
 #include "attn_rows.h"
 
-template <int DH, typename KT, bool SHARED>
-__global__ __launch_bounds__(256) void k_rows_wave(RowsArgs a)
+// ---- single tokens ---------------------------------------------------------------
+
+// Work-group (16 query heads of a kv head, slot): the piece of that slot, or
+// item `slot` whole where there are no balanced ranges.
+template <int DH, typename KT>
+__global__ __launch_bounds__(256) void k_window(RowsArgs a)
 {
 #pragma clang fp contract(off)
-    constexpr int DL = RowState<DH>::DL;
-    const int lane = threadIdx.x & 63;
-    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (long)a.n * a.n_heads) return;
-    const int i = (int)(row / a.n_heads), h = (int)(row % a.n_heads), kvh = h / (a.n_heads / a.n_kv);
-    const bool on = lane * DL < DH;
-    RowState<DH> r;
-    r.m = -INFINITY;
-    r.l = 0.0f;
-    const size_t at = (size_t)row * DH + (on ? lane * DL : 0);
-#pragma unroll
-    for (int d = 0; d < DL; d++) {
-        r.q[d] = a.q[at + d];
-        r.o[d] = 0.0f;
+    __shared__ RowsMeet<DH> meet;
+    const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
+    const int kvh = blockIdx.x / blocks, r0 = (blockIdx.x % blocks) * 16, slot = blockIdx.y;
+    const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int i = slot, u0 = 0, u1 = 0;
+    bool whole = true;
+    if (a.bal) {
+        i = rows_piece(a, slot, &u0, &u1, &whole);
+        if (i < 0) return;
     }
     size_t base;
     const int L = rows_item(a, i, &base);
+    const RowsLine line = rows_line(L - 1, L - 1, a.window, a.sinks);
+    if (!a.bal) u1 = L > 0 ? line.tiles() : 0;
+    const size_t row0 = (size_t)i * a.n_heads + (size_t)kvh * G;
+    RowsWave<DH, KT, 1> w;
+    w.start([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     base += (size_t)kvh * a.max_ctx * DH;
-    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
-    int seen = L;
-    if constexpr (SHARED) {
-        const size_t pb = (size_t)kvh * a.prefix_ctx * DH;
-        row_walk<DH, KT>(r, (const KT *)a.pk + pb, (const KT *)a.pv + pb, 0, a.prefix);
-        row_walk<DH, KT>(r, k, v, 0, L);
-        seen += a.prefix;
-    } else {
-        const int s = min(a.sinks, L);
-        row_walk<DH, KT>(r, k, v, 0, s);
-        row_walk<DH, KT>(r, k, v, max(s, L - a.window), L);
-    }
-    if (!on) return;
-#pragma unroll
-    for (int d = 0; d < DL; d++) a.out[at + d] = seen > 0 ? r.o[d] / r.l : 0.0f;
+    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, u0 + wid, u1, RW_NW, nullptr);
+    const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
+    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+        r += r0;
+        if (r >= G) return;
+        if (whole) {
+            const float f = L > 0 ? 1.0f / l : 0.0f;
+            for (auto &y : x) y = L > 0 ? y * f : 0.0f;
+            rows_store(a.out + (row0 + r) * DH + d, x);
+        } else {
+            rows_store(a.po + (part + r) * DH + d, x);
+            if (d == 0) {
+                a.pm[part + r] = m;
+                a.pl[part + r] = l;
+            }
+        }
+    });
 }
 
-template <bool SHARED>
-static int launch_rows(const RowsArgs &a, hipStream_t s)
+// One work-group per (query head, item): the item's pieces.
+template <int DH>
+__global__ __launch_bounds__(256) void k_window_merge(RowsArgs a)
 {
-    const dim3 grid((unsigned)(((long)a.n * a.n_heads + 3) / 4)), block(256);
-#define ROWS(DHV)                                                                                        \
-    if (a.kv_f16) hipLaunchKernelGGL((k_rows_wave<DHV, _Float16, SHARED>), grid, block, 0, s, a);        \
-    else hipLaunchKernelGGL((k_rows_wave<DHV, float, SHARED>), grid, block, 0, s, a);
-    switch (a.d_head) {
-    case 16: ROWS(16); break;
-    case 32: ROWS(32); break;
-    case 64: ROWS(64); break;
-    case 128: ROWS(128); break;
-    case 256: ROWS(256); break;
-    default: return -4;
+    constexpr int LPR = DH / 4;
+    const int G = a.n_heads / a.n_kv, h = blockIdx.x, kvh = h / G, i = blockIdx.y, tid = threadIdx.x;
+    int first;
+    const int np = rows_pieces(a, i, &first);
+    if (np == 1) return;   // finished by its only piece
+    const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
+    const f32x4 o = rows_sum<DH, 256 / LPR>(np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
+        const size_t at = p0 + (size_t)j * G;
+        *m = a.pm + at;
+        *l = a.pl + at;
+        *x = a.po + at * DH;
+    });
+    if (tid < LPR) *(f32x4 *)(a.out + ((size_t)i * a.n_heads + h) * DH + 4 * tid) = o;
+}
+
+// ---- prompts ---------------------------------------------------------------------
+
+// Rows of a kv head are (token, head of the group), token-major, in blocks of
+// 16 RT; work-group (block and kv head, part) walks its part of the tiles that the
+// block's tokens see between them.
+template <int DH, typename KT, int RT>
+__global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
+{
+#pragma clang fp contract(off)
+    __shared__ RowsMeet<DH> meet;
+    __shared__ int odd;
+    const int G = a.n_heads / a.n_kv, rows = a.n * G;
+    const int kvh = blockIdx.x % a.n_kv, r0 = blockIdx.x / a.n_kv * 16 * RT, part = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nr = min(16 * RT, rows - r0);
+    RowsSeen seen;
+    seen.first = a.pos0 + r0 / G;
+    seen.last = a.pos0 + (r0 + nr - 1) / G;
+    seen.window = a.window;
+    seen.sinks = a.sinks;
+    const RowsLine line = rows_line(seen.first, seen.last, a.window, a.sinks);
+    const int T = line.tiles(), R = (T + a.parts - 1) / a.parts;
+    const int u0 = min(part * R, T), u1 = min(u0 + R, T);
+    int pos[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) pos[rt] = a.pos0 + min(r0 + 16 * rt + (lane & 15), rows - 1) / G;
+    seen.pos = pos;
+    auto row_at = [&](int r) {   // of q and out
+        r = min(r0 + r, rows - 1);
+        return (size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G;
+    };
+    const size_t base = (size_t)kvh * a.max_ctx * DH;
+    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
+    RowsWave<DH, KT, RT> w;
+    w.start([&](int r) { return a.q + row_at(r) * DH; });
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    rows_walk<DH, KT, RT, true>(w, k, v, line, u0 + wid, u1, RW_NW, &seen);
+    const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
+    bool bad = false;
+    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+        if (r >= nr) return;
+        float z = 0.0f;
+        for (auto &y : x) z += y * 0.0f;
+        bad |= !(z == 0.0f);
+        if (a.parts == 1) {
+            const float f = 1.0f / l;
+            for (auto &y : x) y *= f;
+            rows_store(a.out + row_at(r) * DH + d, x);
+        } else {
+            const size_t at = x0 + (size_t)r * a.parts;
+            rows_store(a.xo + at * DH + d, x);
+            if (d == 0) {
+                a.xm[at] = m;
+                a.xl[at] = l;
+            }
+        }
+    });
+    // A masked position is in its tile's products with weight 0, which a V row
+    // that is not finite turns into NaN for the rows that do not see it: where
+    // an output is not finite, the block's rows are walked again one by one.
+    if (bad) odd = 1;
+    __syncthreads();
+    if (!odd) return;
+    constexpr int DL = RowState<DH>::DL;
+    const bool on = lane * DL < DH;
+    for (int r = wid; r < nr; r += RW_NW) {
+        const size_t qa = row_at(r) * DH + (on ? lane * DL : 0);
+        const int p = a.pos0 + (r0 + r) / G;
+        RowState<DH> t;
+        t.m = -INFINITY;
+        t.l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DL; d++) {
+            t.q[d] = a.q[qa + d];
+            t.o[d] = 0.0f;
+        }
+        for (int u = u0; u < u1; u++) {
+            int p0, cnt;
+            line.tile(u, &p0, &cnt);
+            const int end = min(p0 + cnt, p + 1), lo = p + 1 - a.window;
+            row_walk<DH, KT>(t, k, v, p0, min(end, a.sinks));
+            row_walk<DH, KT>(t, k, v, max(max(p0, lo), min(a.sinks, end)), end);
+        }
+        if (!on) continue;
+        const size_t at = x0 + (size_t)r * a.parts;
+#pragma unroll
+        for (int d = 0; d < DL; d++) {
+            if (a.parts == 1) a.out[qa + d] = t.o[d] / t.l;
+            else a.xo[at * DH + lane * DL + d] = t.o[d];
+        }
+        if (a.parts > 1 && lane == 0) {
+            a.xm[at] = t.m;
+            a.xl[at] = t.l;
+        }
     }
-#undef ROWS
+}
+
+// The parts of (query head, token) rows, a lane per four dimensions.
+template <int DH>
+__global__ __launch_bounds__(256) void k_window_prompt_merge(RowsArgs a)
+{
+    constexpr int LPR = DH / 4;
+    const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;   // of out
+    if (row >= (size_t)a.n * a.n_heads) return;
+    const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
+    const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
+    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
+        *m = a.xm + x0 + j;
+        *l = a.xl + x0 + j;
+        *x = a.xo + (x0 + j) * DH;
+    });
+    *(f32x4 *)(a.out + row * DH + 4 * d4) = o;
+}
+
+// ---- plans and launches ------------------------------------------------------------
+
+// Most tiles of a token's line.
+static long span_tiles(int max_ctx, int window, int sinks)
+{
+    const long w = std::min(window, max_ctx), s = std::min(sinks, max_ctx);
+    return std::min((long)ceil_div(w, RW_TP) + ceil_div(s, RW_TP), (long)ceil_div(max_ctx, RW_TP) + 2);
+}
+
+int rows_plan_bal(int n, long heads, long span)
+{
+    if (span <= 2 * RW_NW || n * heads >= RW_WGS || n * (span + RW_PAD) > INT32_MAX) return 0;
+    const long want = std::max(1L, RW_WGS / heads - n);
+    return (int)std::min(want, n * (long)ceil_div(span + RW_PAD, RW_RMIN));
+}
+
+RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks)
+{
+    RowsPlan p;
+    const int G = n_heads / n_kv;
+    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks));
+    if (p.bal) p.pieces = (size_t)n_kv * (p.bal + n) * G;
+    return p;
+}
+
+static int prompt_tiles(int n, int G) { return (long)n * G <= 16 ? 1 : (long)n * G <= 32 ? 2 : 4; }
+static int prompt_rt(int n, int G, int d_head, int kv_f16)
+{
+    return std::min(prompt_tiles(n, G), d_head == 256 ? 1 : kv_f16 && d_head < 128 ? 4 : 2);
+}
+
+static int prompt_parts(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks, int rt)
+{
+    const int G = n_heads / n_kv;
+    const long blocks = (long)n_kv * ceil_div((long)n * G, 16 * rt);
+    const long span = std::min(span_tiles(max_ctx, window, sinks) + ceil_div(16 * rt, G * RW_TP) + 1, (long)ceil_div(max_ctx, RW_TP) + 2);
+    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(span, 2 * RW_NW)));
+}
+
+RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
+{
+    RowsPlan p;
+    const int G = n_heads / n_kv;
+    for (int f16 = 0; f16 < 2; f16++)
+        p.parts = std::max(p.parts, prompt_parts(n, n_heads, n_kv, max_ctx, window, sinks, prompt_rt(n, G, d_head, f16)));
+    if (p.parts > 1) p.cross = (size_t)n * n_heads * p.parts;
+    return p;
+}
+
+int launch_attn_window(const RowsArgs &a, hipStream_t s)
+{
+    const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), a.bal + a.n), block(256);
+#define WIN(DH)                                                                          \
+    if (a.kv_f16) hipLaunchKernelGGL((k_window<DH, _Float16>), grid, block, 0, s, a);    \
+    else hipLaunchKernelGGL((k_window<DH, float>), grid, block, 0, s, a);
+    RW_BY_D_HEAD(a.d_head, WIN)
+#undef WIN
+    if (a.bal) {
+#define MERGE(DH) hipLaunchKernelGGL(k_window_merge<DH>, dim3(a.n_heads, a.n), block, 0, s, a);
+        RW_BY_D_HEAD(a.d_head, MERGE)
+#undef MERGE
+    }
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
 
-int launch_attn_window(const RowsArgs &a, hipStream_t s) { return launch_rows<false>(a, s); }
-int launch_attn_shared(const RowsArgs &a, hipStream_t s) { return launch_rows<true>(a, s); }
+int launch_attn_window_prompt(const RowsArgs &a0, hipStream_t s)
+{
+    RowsArgs a = a0;
+    const int G = a.n_heads / a.n_kv, rt = prompt_rt(a.n, G, a.d_head, a.kv_f16);
+    a.parts = std::min(a.parts, prompt_parts(a.n, a.n_heads, a.n_kv, a.max_ctx, a.window, a.sinks, rt));
+    const dim3 grid(a.n_kv * ceil_div((long)a.n * G, 16 * rt), a.parts), block(256);
+#define LAUNCH(DH, KT, RT) hipLaunchKernelGGL((k_window_prompt<DH, KT, RT>), grid, block, 0, s, a)
+#define PRO(DH)                                                                  \
+    if (rt == 1) { if (a.kv_f16) LAUNCH(DH, _Float16, 1); else LAUNCH(DH, float, 1); }  \
+    else if constexpr (DH < 256) {                                               \
+        if (a.kv_f16) { if (rt == 2) LAUNCH(DH, _Float16, 2); else LAUNCH(DH, _Float16, 4); }  \
+        else LAUNCH(DH, float, 2);                                               \
+    }
+    RW_BY_D_HEAD(a.d_head, PRO)
+#undef PRO
+#undef LAUNCH
+    if (a.parts > 1) {
+#define MERGE(DH)                                                                                             \
+    hipLaunchKernelGGL(k_window_prompt_merge<DH>, dim3((unsigned)(((size_t)a.n * a.n_heads * DH + 1023) / 1024)), block, 0, s, a);
+        RW_BY_D_HEAD(a.d_head, MERGE)
+#undef MERGE
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -4;
+}

@@ -595,38 +595,48 @@ bool rows_shape(int n, int n_heads, int n_kv, int d_head, int max_ctx, int *rc)
 {
     *rc = E_ARGS;
     if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_kv > 65535 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
-    if (d_head < 1 || (size_t)n_heads * d_head > INT32_MAX) return false;
+    if (d_head < 1 || (size_t)n_heads * d_head > INT32_MAX || (size_t)n * n_heads > INT32_MAX) return false;
     *rc = E_UNSUPPORTED;
     if (d_head != 16 && d_head != 32 && d_head != 64 && d_head != 128 && d_head != 256) return false;
     *rc = E_OK;
     return true;
 }
 
-size_t window_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int *rc)
+// Workspace of a plan: (m, l, o[d_head]) per partial result.
+size_t plan_bytes(const RowsPlan &p, int d_head)
+{
+    return align_up((p.pieces + p.cross) * (d_head + 2) * sizeof(float), ALIGN) + ALIGN;
+}
+
+size_t window_bytes(bool prompt, int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks,
+                    RowsPlan *p, int *rc)
 {
     if (!rows_shape(n, n_heads, n_kv, d_head, max_ctx, rc)) return 0;
-    if (window < 1 || sinks < 0) {
+    if (window < 1 || sinks < 0 || (prompt && n > max_ctx)) {
         *rc = E_ARGS;
         return 0;
     }
-    return ALIGN;
+    *p = prompt ? rows_plan_prompt(n, n_heads, n_kv, d_head, max_ctx, window, sinks)
+                : rows_plan_window(n, n_heads, n_kv, max_ctx, window, sinks);
+    return plan_bytes(*p, d_head);
 }
 
-size_t shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx, int *rc)
+size_t shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx, RowsPlan *p, int *rc)
 {
     if (!rows_shape(n, n_heads, n_kv, d_head, max_ctx, rc)) return 0;
     if (prefix_len < 0) {
         *rc = E_ARGS;
         return 0;
     }
-    return ALIGN;
+    *p = rows_plan_shared(n, n_heads, n_kv, d_head, prefix_len, max_ctx);
+    return plan_bytes(*p, d_head);
 }
 
 // What the attention calls share: pointers and workspace checked, arguments
 // laid out (`need`: the workspace size, 0 a refusal already in *rc).
 bool rows_args(RowsArgs &a, cmolhip_ctx_t *c, int n, const float *q, const void *k, const void *v, const int32_t *slots,
-               size_t slot_stride, int n_heads, int n_kv, int d_head, int max_ctx, int kv_f16, const void *ws,
-               size_t ws_bytes, size_t need, float *out, int *rc)
+               size_t slot_stride, int n_heads, int n_kv, int d_head, int max_ctx, int kv_f16, void *ws,
+               size_t ws_bytes, size_t need, const RowsPlan &p, float *out, int *rc)
 {
     if (!need) return false;
     *rc = E_ARGS;
@@ -647,6 +657,14 @@ bool rows_args(RowsArgs &a, cmolhip_ctx_t *c, int n, const float *q, const void 
     a.d_head = d_head;
     a.max_ctx = max_ctx;
     a.kv_f16 = kv_f16 != 0;
+    a.bal = p.bal;
+    a.parts = p.parts;
+    a.po = (float *)ws;
+    a.xo = a.po + p.pieces * d_head;
+    a.pm = a.xo + p.cross * d_head;
+    a.pl = a.pm + p.pieces;
+    a.xm = a.pl + p.pieces;
+    a.xl = a.xm + p.cross;
     return true;
 }
 
@@ -657,7 +675,8 @@ extern "C" {
 size_t cmolhip_attn_window_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
 {
     int rc;
-    return window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
+    RowsPlan p;
+    return window_bytes(false, n, n_heads, n_kv, d_head, max_ctx, window, sinks, &p, &rc);
 }
 
 int cmolhip_attn_window(cmolhip_ctx_t *c, int n, const float *q, const void *kcache, const void *vcache,
@@ -666,9 +685,10 @@ int cmolhip_attn_window(cmolhip_ctx_t *c, int n, const float *q, const void *kca
 {
     int rc;
     RowsArgs a{};
-    const size_t need = window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
+    RowsPlan p;
+    const size_t need = window_bytes(false, n, n_heads, n_kv, d_head, max_ctx, window, sinks, &p, &rc);
     if (!rows_args(a, c, n, q, kcache, vcache, slots, slot_stride, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes,
-                   need, out, &rc))
+                   need, p, out, &rc))
         return rc;
     if (!seqlen) return E_ARGS;
     a.seqlen = seqlen;
@@ -681,7 +701,8 @@ int cmolhip_attn_window(cmolhip_ctx_t *c, int n, const float *q, const void *kca
 size_t cmolhip_attn_window_prompt_bytes(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
 {
     int rc;
-    return n <= max_ctx ? window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc) : 0;
+    RowsPlan p;
+    return window_bytes(true, n, n_heads, n_kv, d_head, max_ctx, window, sinks, &p, &rc);
 }
 
 int cmolhip_attn_window_prompt(cmolhip_ctx_t *c, int n, int pos0, const float *q, const void *kcache, const void *vcache,
@@ -690,22 +711,24 @@ int cmolhip_attn_window_prompt(cmolhip_ctx_t *c, int n, int pos0, const float *q
 {
     int rc;
     RowsArgs a{};
-    const size_t need = window_bytes(n, n_heads, n_kv, d_head, max_ctx, window, sinks, &rc);
-    if (need && (pos0 < 0 || n > max_ctx || pos0 > max_ctx - n)) return E_ARGS;
-    if (!rows_args(a, c, n, q, kcache, vcache, nullptr, 0, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes, need,
+    RowsPlan p;
+    const size_t need = window_bytes(true, n, n_heads, n_kv, d_head, max_ctx, window, sinks, &p, &rc);
+    if (need && (pos0 < 0 || pos0 > max_ctx - n)) return E_ARGS;
+    if (!rows_args(a, c, n, q, kcache, vcache, nullptr, 0, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes, need, p,
                    out, &rc))
         return rc;
     a.pos0 = pos0;
     a.window = std::min(window, max_ctx);
     a.sinks = std::min(sinks, max_ctx);
     OnDevice on(c->device);
-    return on.ok ? launch_attn_window(a, c->stream) : E_INVALID;
+    return on.ok ? launch_attn_window_prompt(a, c->stream) : E_INVALID;
 }
 
 size_t cmolhip_attn_shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx)
 {
     int rc;
-    return shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &rc);
+    RowsPlan p;
+    return shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &p, &rc);
 }
 
 int cmolhip_attn_shared(cmolhip_ctx_t *c, int n, const float *q, const void *kprefix, const void *vprefix,
@@ -715,9 +738,10 @@ int cmolhip_attn_shared(cmolhip_ctx_t *c, int n, const float *q, const void *kpr
 {
     int rc;
     RowsArgs a{};
-    const size_t need = shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &rc);
+    RowsPlan p;
+    const size_t need = shared_bytes(n, n_heads, n_kv, d_head, prefix_len, max_ctx, &p, &rc);
     if (!rows_args(a, c, n, q, kcache, vcache, slots, slot_stride, n_heads, n_kv, d_head, max_ctx, kv_f16, ws, ws_bytes,
-                   need, out, &rc))
+                   need, p, out, &rc))
         return rc;
     if (!seqlen || prefix_len > prefix_ctx || (prefix_len && (!kprefix || !vprefix))) return E_ARGS;
     if (!aligned16(kprefix) || !aligned16(vprefix)) return E_ARGS;
