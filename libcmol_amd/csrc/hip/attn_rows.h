@@ -59,6 +59,7 @@ struct RowsArgs {
     int parts;                 // parts of the prefix, or of a prompt block's positions
     float *pm, *pl, *po;       // [n_kv][bal + n][G]
     float *xm, *xl, *xo;       // [n_kv][n * G][parts]
+    void *split;               // prompt over an fp32 cache: its f16 pairs (attn_wprompt.hip)
 };
 
 // ---- which positions -----------------------------------------------------------
@@ -624,6 +625,7 @@ int rows_plan_bal(int n, long heads, long span);
 struct RowsPlan {
     int bal = 0, parts = 0;
     size_t pieces = 0, cross = 0;   // pm / pl / po, and xm / xl / xo
+    size_t split = 0;               // bytes of the f16 pairs
 };
 RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks);
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks);
@@ -632,6 +634,13 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
 int launch_attn_window(const RowsArgs &a, hipStream_t s);
 int launch_attn_window_prompt(const RowsArgs &a, hipStream_t s);
 int launch_attn_shared(const RowsArgs &a, hipStream_t s);
+int launch_prompt_parts(const RowsArgs &a, hipStream_t s);   // merge of a prompt's parts (a.parts > 1)
+
+// Prompts whose query rows share the positions through LDS (attn_wprompt.hip).
+bool wprompt_takes(int n, int n_heads, int n_kv, int d_head);
+int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16);
+size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window, int sinks);
+int launch_wprompt(const RowsArgs &a, hipStream_t s);
 
 #define RW_BY_D_HEAD(d, F)          \
     switch (d) {                    \

@@ -164,23 +164,6 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     }
 }
 
-// The parts of (query head, token) rows, a lane per four dimensions.
-template <int DH>
-__global__ __launch_bounds__(256) void k_window_prompt_merge(RowsArgs a)
-{
-    constexpr int LPR = DH / 4;
-    const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;   // of out
-    if (row >= (size_t)a.n * a.n_heads) return;
-    const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
-    const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
-    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
-        *m = a.xm + x0 + j;
-        *l = a.xl + x0 + j;
-        *x = a.xo + (x0 + j) * DH;
-    });
-    *(f32x4 *)(a.out + row * DH + 4 * d4) = o;
-}
-
 // ---- plans and launches ------------------------------------------------------------
 
 // Most tiles of a token's line.
@@ -224,8 +207,11 @@ RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx,
 {
     RowsPlan p;
     const int G = n_heads / n_kv;
+    const bool lds = wprompt_takes(n, n_heads, n_kv, d_head);
     for (int f16 = 0; f16 < 2; f16++)
-        p.parts = std::max(p.parts, prompt_parts(n, n_heads, n_kv, max_ctx, window, sinks, prompt_rt(n, G, d_head, f16)));
+        p.parts = std::max(p.parts, lds ? wprompt_parts(n, n_heads, n_kv, d_head, max_ctx, window, sinks, f16)
+                                        : prompt_parts(n, n_heads, n_kv, max_ctx, window, sinks, prompt_rt(n, G, d_head, f16)));
+    if (lds) p.split = wprompt_split_bytes(n, n_kv, d_head, max_ctx, window, sinks);
     if (p.parts > 1) p.cross = (size_t)n * n_heads * p.parts;
     return p;
 }
@@ -249,6 +235,7 @@ int launch_attn_window(const RowsArgs &a, hipStream_t s)
 int launch_attn_window_prompt(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
+    if (wprompt_takes(a.n, a.n_heads, a.n_kv, a.d_head)) return launch_wprompt(a, s);
     const int G = a.n_heads / a.n_kv, rt = prompt_rt(a.n, G, a.d_head, a.kv_f16);
     a.parts = std::min(a.parts, prompt_parts(a.n, a.n_heads, a.n_kv, a.max_ctx, a.window, a.sinks, rt));
     const dim3 grid(a.n_kv * ceil_div((long)a.n * G, 16 * rt), a.parts), block(256);
@@ -262,11 +249,6 @@ int launch_attn_window_prompt(const RowsArgs &a0, hipStream_t s)
     RW_BY_D_HEAD(a.d_head, PRO)
 #undef PRO
 #undef LAUNCH
-    if (a.parts > 1) {
-#define MERGE(DH)                                                                                             \
-    hipLaunchKernelGGL(k_window_prompt_merge<DH>, dim3((unsigned)(((size_t)a.n * a.n_heads * DH + 1023) / 1024)), block, 0, s, a);
-        RW_BY_D_HEAD(a.d_head, MERGE)
-#undef MERGE
-    }
+    if (a.parts > 1 && launch_prompt_parts(a, s)) return -4;
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }

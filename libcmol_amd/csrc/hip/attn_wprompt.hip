@@ -1,0 +1,572 @@
+// attn_wprompt.hip — windowed attention of prompts (attn_rows.h) at d_head 64
+// and 128, where there are enough query rows to share the cached positions
+// through LDS.
+//
+// Rows of a kv head are (token, head of the group), token-major.  A work-group
+// of eight waves takes 128 of them and a part of the tiles of TP positions that
+// their tokens see between them; the waves of one half walk every second tile,
+// wave w4 of a half owns rows 32 w4 .. +31 (two tiles of 16), and the halves'
+// softmaxes and outputs meet at the end.  The next two tiles are copied into
+// LDS by direct-to-LDS loads while the present ones are used.
+//   fp16 cache (TP = 64): K pieces of 1 KiB in the operand's order (16 positions
+//     x 32 dimensions, gathered by the loads' addresses), V rows as cached, their
+//     32-byte units XOR-swizzled by the row for the transposing reads
+//     (ds_read_b64_tr_b16) of the second product.
+//   fp32 cache (TP = 32): k_prompt_split lays the positions the prompt sees out
+//     once per call as f16 pairs (x = hi + lo), both operands in their order.
+//     A tile is scaled by a power of two that puts its largest |K| (|V|) into
+//     [2^9, 2^10), so hi and lo are normal f16 numbers whatever the cache's
+//     range: 22 bits of a value, 2^-33 of the tile's largest below.  The score
+//     takes K's exponent back into its exponential, the weights V's.
+// Products are exact (lo.lo, below 2^-22 of each, is left out over fp32), sums
+// fp32; the query is split as the walk's of attn_rows.h, the weights too.
+// A tile has 2 x 2 (fp32 3) products per (row tile, 16 positions, 32
+// dimensions): bound by the matrix pipe and by the softmax's vector
+// instructions beside it.
+#include "attn_rows.h"
+#include "lds_limit.h"
+
+constexpr int WP_NT = 512, WP_ROWS = 128, WP_TS = 32;   // threads, rows, positions of a split tile
+
+// Tiles of TP positions that a prompt's tokens see: `ns` of sinks, then the
+// run from lo (where the sinks reach into it, one run from 0).
+struct PromptTiles {
+    int s, lo, ns;
+    __host__ __device__ PromptTiles(int pos0, int window, int sinks, int tp)
+    {
+        lo = pos0 + 1 > window ? pos0 + 1 - window : 0;
+        s = sinks;
+        if (sinks > lo) s = lo = 0;
+        ns = (s + tp - 1) / tp;
+    }
+    __host__ __device__ int count(int last, int tp) const { return ns + (last + tp - lo) / tp; }
+};
+
+// A split tile: K hi and lo pieces, V hi and lo pieces, WP_TS positions.
+template <int DH>
+constexpr int wp_tile_halves() { return WP_TS * DH * 4; }
+
+template <int DH>
+__global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst, int *exps, int tiles)
+{
+#pragma clang fp contract(off)
+    constexpr int KS = DH / 32, DT = DH / 16, NK = 2 * KS * 64 / 256, NV = DT * 64 / 256, TH = wp_tile_halves<DH>();
+    __shared__ float top[2][4];
+    const int tile = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
+    const PromptTiles pt(a.pos0, a.window, a.sinks, WP_TS);
+    const int p0 = tile < pt.ns ? tile * WP_TS : pt.lo + (tile - pt.ns) * WP_TS;
+    const int cnt = min(WP_TS, (tile < pt.ns ? pt.s : a.pos0 + a.n) - p0);
+    const size_t base = ((size_t)kvh * a.max_ctx + p0) * DH;
+    const float *kb = (const float *)a.k + base, *vb = (const float *)a.v + base;
+    dst += ((size_t)kvh * tiles + tile) * TH;
+    float k[NK][8], v[NV][8], tk = 0.0f, tv = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NK; j++) {
+        const int it = tid + 256 * j, lane = it & 63, cs = it >> 6, c = cs / KS, s = cs % KS, p = 16 * c + (lane & 15);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const f32x4 x = p < cnt ? *(const f32x4 *)(kb + (size_t)p * DH + 32 * s + 8 * (lane >> 4) + 4 * h) : f32x4{};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                k[j][4 * h + e] = x[e];
+                if (fabsf(x[e]) < INFINITY) tk = fmaxf(tk, fabsf(x[e]));
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int it = tid + 256 * j, lane = it & 63, t = it >> 6, g = lane >> 4;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int p = (e < 4 ? 0 : 12) + 4 * g + e;
+            v[j][e] = p < cnt ? vb[(size_t)p * DH + 16 * t + (lane & 15)] : 0.0f;
+            if (fabsf(v[j][e]) < INFINITY) tv = fmaxf(tv, fabsf(v[j][e]));
+        }
+    }
+    tk = wave_max(tk);
+    tv = wave_max(tv);
+    if ((tid & 63) == 0) {
+        top[0][tid >> 6] = tk;
+        top[1][tid >> 6] = tv;
+    }
+    __syncthreads();
+    int ex[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const float t = fmaxf(fmaxf(top[i][0], top[i][1]), fmaxf(top[i][2], top[i][3]));
+        ex[i] = t > 0.0f ? max(ilogbf(t), -100) - 9 : 0;
+        if (tid == 0) exps[((size_t)kvh * tiles + tile) * 2 + i] = ex[i];
+    }
+    auto put = [&](const float (&x)[8], int e, _Float16 *at) {
+        f16x8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float y = ldexpf(x[i], -e);
+            hi[i] = (_Float16)y;
+            lo[i] = (_Float16)(y - (float)hi[i]);
+        }
+        *(f16x8 *)at = hi;
+        *(f16x8 *)(at + 512) = lo;
+    };
+#pragma unroll
+    for (int j = 0; j < NK; j++) {
+        const int it = tid + 256 * j;
+        put(k[j], ex[0], dst + (it >> 6) * 1024 + (it & 63) * 8);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+        const int it = tid + 256 * j;
+        put(v[j], ex[1], dst + TH / 2 + (it >> 6) * 1024 + (it & 63) * 8);
+    }
+}
+
+template <int DH, bool F16>
+__global__ __launch_bounds__(WP_NT) __attribute__((amdgpu_waves_per_eu(2)))
+void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles)
+{
+#pragma clang fp contract(off)
+    typedef typename std::conditional<F16, _Float16, float>::type KT;
+    constexpr int TP = F16 ? 64 : WP_TS, CT = TP / 16, RT = 2;
+    constexpr int KS = DH / 32, DT = DH / 16;
+    constexpr int KB = F16 ? TP * DH * 2 : wp_tile_halves<DH>();   // K bytes of a tile (V: as many)
+    constexpr int TILE = 2 * KB;
+    constexpr int RPP = 1024 / (2 * DH);              // fp16: V rows per 1 KiB piece
+    constexpr int VPW = TP / RPP / 4;                 // fp16: V pieces per wave
+    constexpr int PIECES = TILE / 1024 / 4;           // fp32: pieces per wave
+    extern __shared__ __attribute__((aligned(256))) uint8_t smem_w[];   // [stage][half][TILE]
+    __shared__ int odd;
+
+    const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), half = wid >> 2, w4 = wid & 3;
+    const int G = a.n_heads / a.n_kv, rows = a.n * G;
+    const int blocks = gridDim.x / a.n_kv;
+    // the blocks of the longest lines first
+    const int kvh = blockIdx.x % a.n_kv, r0 = (blocks - 1 - (int)(blockIdx.x / a.n_kv)) * WP_ROWS, part = blockIdx.y;
+    const int nr = min(WP_ROWS, rows - r0);
+    const int first = a.pos0 + r0 / G, last = a.pos0 + (r0 + nr - 1) / G;
+    // the block's tiles: [0, na) and [nb, ne)
+    const PromptTiles pt(a.pos0, a.window, a.sinks, TP);
+    const int lo = max(first + 1 - a.window, 0);
+    const int na = pt.s || !a.sinks ? pt.ns : (min(a.sinks, lo) + TP - 1) / TP;
+    const int nb = max(pt.ns + (lo - pt.lo) / TP, na), ne = pt.count(last, TP);
+    const int T = na + ne - nb, R = ((T + a.parts - 1) / a.parts + 1) & ~1;   // (pairs of tiles)
+    const int u0 = min(part * R, T), u1 = min(u0 + R, T);
+    auto tile = [&](int u) { return u < na ? u : u - na + nb; };
+    auto start = [&](int t) { return t < pt.ns ? t * TP : pt.lo + (t - pt.ns) * TP; };
+    auto limit = [&](int t) { return t < pt.ns ? pt.s : last + 1; };
+
+    const size_t base = (size_t)kvh * a.max_ctx * DH;
+    const uint8_t *kb = (const uint8_t *)uniform_ptr((const KT *)a.k + base);
+    const uint8_t *vbp = (const uint8_t *)uniform_ptr((const KT *)a.v + base);
+    const uint8_t *sb = (const uint8_t *)uniform_ptr(split + (size_t)kvh * tiles * wp_tile_halves<DH>());
+    const int *ex = uniform_ptr(exps + (size_t)kvh * tiles * 2);
+    const int vrow = lane / (DH / 8), vch = lane % (DH / 8);
+    auto issue = [&](int st, int u) {
+        uint8_t *dst = smem_w + (st * 2 + half) * TILE;
+        const int t = tile(u);
+        if constexpr (F16) {
+            const int p0 = start(t), cnt = limit(t) - p0;   // (past it: its last position again)
+            const uint8_t *ks = kb + (size_t)p0 * (2 * DH), *vs = vbp + (size_t)p0 * (2 * DH);
+            const uint32_t kp = (uint32_t)min(16 * w4 + col, cnt - 1) * (2 * DH) + 16 * g;
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(ks + kp + 64 * s), (lvoid_t *)(dst + (w4 * KS + s) * 1024),
+                                                 16, 0, 0);
+#pragma unroll
+            for (int i = 0; i < VPW; i++) {
+                const int r = (w4 * VPW + i) * RPP + vrow;   // row of the tile
+                const int f = DH == 128 ? r & 7 : (r >> 1) & 3;
+                const uint32_t vp = (uint32_t)min(r, cnt - 1) * (2 * DH) + 32 * ((vch >> 1) ^ f) + 16 * (vch & 1);
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(vs + vp),
+                                                 (lvoid_t *)(dst + KB + (w4 * VPW + i) * 1024), 16, 0, 0);
+            }
+        } else {
+            const uint8_t *src = sb + (size_t)t * TILE;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const int pc = w4 * PIECES + i;
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(src + pc * 1024 + lane * 16),
+                                                 (lvoid_t *)(dst + pc * 1024), 16, 0, 0);
+            }
+        }
+    };
+    if (u0 + half < u1) issue(0, u0 + half);
+
+    auto row_at = [&](int r) {   // of q and out
+        r = min(r0 + r, rows - 1);
+        return (size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G;
+    };
+    // query operands of rows 32 w4 + 16 rt + col: the row's largest into [2^9, 2^10)
+    f16x8 qh[RT][KS], ql[RT][KS];
+    float c2[RT];
+    int pos[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int r = 32 * w4 + 16 * rt + col;
+        pos[rt] = a.pos0 + min(r0 + r, rows - 1) / G;
+        const float *q = a.q + row_at(r) * DH + 8 * g;
+        float x[KS][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const f32x4 y0 = ldg((const f32x4 *)(q + 32 * s)), y1 = ldg((const f32x4 *)(q + 32 * s + 4));
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[s][e] = e < 4 ? y0[e & 3] : y1[e & 3];
+                top = fmaxf(top, fabsf(x[s][e]));
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const int e0 = top > 0.0f && top < INFINITY ? max(ilogbf(top), -100) - 9 : 0;
+        c2[rt] = ldexpf(1.44269504088896341f / sqrtf((float)DH), e0);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float y = ldexpf(x[s][e], -e0);
+                qh[rt][s][e] = (_Float16)y;
+                ql[rt][s][e] = (_Float16)(y - (float)qh[rt][s][e]);
+            }
+    }
+    // the largest exponent of V among the part's tiles: the outputs' unit
+    int ve = 0;
+    if constexpr (!F16) {
+        ve = -1000;
+        for (int u = u0 + lane; u < u1; u += 64) ve = max(ve, ex[2 * tile(u) + 1]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) ve = max(ve, __shfl_xor(ve, o, 64));
+        ve = __builtin_amdgcn_readfirstlane(ve);
+    }
+    const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 o[RT][DT];
+    float m[RT], mk[RT], l[RT];   // m: reference in log2 units; mk = RW_SCALE - m
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY;
+        mk[rt] = RW_SCALE;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int t = 0; t < DT; t++) o[rt][t] = zero4;
+    }
+    // fp16: transposing reads, this lane's bytes of row 4g + col/4 (+ 16 per c)
+    // of dimension tile t at vaddr ^ 32t
+    const int vr = 4 * g + (col >> 2);
+    const uint32_t vaddr = (uint32_t)(vr * (2 * DH) + 32 * (DH == 128 ? vr & 7 : (vr >> 1) & 3) + 8 * (col & 3));
+
+    int st = 0;
+    for (int uu = u0; uu < u1; uu += 2, st ^= 1) {
+        const int u = uu + half;
+        // the tiles have landed and every wave is done with the other stage
+        __builtin_amdgcn_s_waitcnt(WAITCNT_VM_LGKM0(0));
+        __syncthreads();
+        if (u + 2 < u1) issue(st ^ 1, u + 2);
+        if (u >= u1) continue;   // (the last pair may be one tile)
+        const uint8_t *ks_ = smem_w + (st * 2 + half) * TILE, *vs_ = ks_ + KB;
+        const int t = tile(u), p0 = start(t), cnt = limit(t) - p0;
+        float kf = 1.0f, vf = 1.0f;
+        if constexpr (!F16) {
+            kf = ldexpf(1.0f, ex[2 * t]);
+            vf = ldexpf(1.0f, ex[2 * t + 1] - ve);
+        }
+        // ---- scores: sc[rt][c][i] = position p0 + 16c + 4g + i of row col
+        float sc[RT][CT][4];
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            f32x4 s1[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) s1[rt] = zero4;
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if constexpr (F16) {
+                    const f16x8 k = *(const f16x8 *)(ks_ + (c * KS + s) * 1024 + lane * 16);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][s], s1[rt], 0, 0, 0);
+                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][s], s1[rt], 0, 0, 0);
+                    }
+                } else {
+                    const f16x8 kh = *(const f16x8 *)(ks_ + (c * KS + s) * 2048 + lane * 16);
+                    const f16x8 kl = *(const f16x8 *)(ks_ + (c * KS + s) * 2048 + 1024 + lane * 16);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[rt][s], s1[rt], 0, 0, 0);
+                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[rt][s], s1[rt], 0, 0, 0);
+                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[rt][s], s1[rt], 0, 0, 0);
+                    }
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sc[rt][c][i] = s1[rt][i];
+        }
+        const int top = p0 + TP - 1;
+        if (top > first || cnt < TP || (top >= a.sinks && p0 <= last - a.window)) {   // uniform
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int at = 16 * c + 4 * g + i, p = p0 + at;
+                        if (at >= cnt || p > pos[rt] || (p >= a.sinks && p <= pos[rt] - a.window)) sc[rt][c][i] = -INFINITY;
+                    }
+        }
+        // ---- online softmax
+        f16x8 ph[RT][CT / 2], pl[RT][CT / 2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            // (above 0: a masked score times it stays -inf)
+            const float f = F16 ? c2[rt] : fmaxf(c2[rt] * kf, 1e-37f);
+            float mx = sc[rt][0][0];
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[rt][c][i]);
+            mx *= f;
+            if (__ballot(mx > m[rt] + RW_LAZY)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m[rt], mx);
+                const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn;
+                const float al = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - mk[rt]);
+                m[rt] = mn;
+                mk[rt] = mkn;
+                l[rt] *= al;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[rt][d] *= al;
+            }
+            float ls = 0.0f;
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], f, mk[rt]));
+                    float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], f, mk[rt]));
+                    ls += e0 + e1;
+                    if constexpr (!F16) {
+                        e0 *= vf;
+                        e1 *= vf;
+                    }
+                    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0, e1));
+                    const f16x2 lw =
+                        __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0 - (float)hi[0], e1 - (float)hi[1]));
+                    ph[rt][c >> 1][4 * (c & 1) + i] = hi[0];
+                    ph[rt][c >> 1][4 * (c & 1) + i + 1] = hi[1];
+                    pl[rt][c >> 1][4 * (c & 1) + i] = lw[0];
+                    pl[rt][c >> 1][4 * (c & 1) + i + 1] = lw[1];
+                }
+            l[rt] += ls;
+        }
+        // ---- O^T += V^T P^T: k-step k covers positions 32k + 4g .. +3 and 32k + 16 + 4g .. +3
+#pragma unroll
+        for (int k = 0; k < CT / 2; k++) {
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                if constexpr (F16) {
+                    typedef short s16x4 __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) s16x4 ls16x4;
+                    const uint8_t *src = vs_ + 32 * k * (2 * DH) + (vaddr ^ (32u * d));
+                    const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)src);
+                    const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)(src + 16 * (2 * DH)));
+                    const f16x8 v = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[rt][k], o[rt][d], 0, 0, 0);
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[rt][k], o[rt][d], 0, 0, 0);
+                    }
+                } else {
+                    const f16x8 vh = *(const f16x8 *)(vs_ + d * 2048 + lane * 16);
+                    const f16x8 vl = *(const f16x8 *)(vs_ + d * 2048 + 1024 + lane * 16);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[rt][k], o[rt][d], 0, 0, 0);
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[rt][k], o[rt][d], 0, 0, 0);
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[rt][k], o[rt][d], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- the halves meet: each finishes one of the two row tiles
+    if (tid == 0) odd = 0;
+    f32x4 *xo = (f32x4 *)smem_w;                              // [half][wave][DT][lane]
+    float *xm = (float *)(smem_w + 8 * DT * 64 * 16);         // [half][wave][lane] m, then l
+    __syncthreads();
+    const int mine = half, other = half ^ 1;                  // row tiles kept and handed over
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) m[rt] = m[rt] == -INFINITY ? -INFINITY : -mk[rt];   // of the weights as they are
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (rt == mine) continue;
+#pragma unroll
+        for (int d = 0; d < DT; d++) xo[((half * 4 + w4) * DT + d) * 64 + lane] = o[rt][d];
+        xm[(half * 4 + w4) * 64 + lane] = m[rt];
+        xm[512 + (half * 4 + w4) * 64 + lane] = l[rt];
+    }
+    __syncthreads();
+    bool bad = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (rt != mine) continue;
+        const int x = (other * 4 + w4) * 64 + lane;
+        const float m1 = xm[x], mm = fmaxf(m[rt], m1), ref = mm == -INFINITY ? 0.0f : mm;
+        const float f0 = __builtin_amdgcn_exp2f(m[rt] - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
+        float ls = l[rt] * f0 + xm[512 + x] * f1;
+        ls += __shfl_xor(ls, 16, 64);
+        ls += __shfl_xor(ls, 32, 64);
+        const int r = 32 * w4 + 16 * rt + col;
+        const bool valid = r < nr;
+        const float unit = ldexpf(1.0f, ve), inv = unit / ls;
+        const size_t at = ((size_t)kvh * rows + min(r0 + r, rows - 1)) * a.parts + part;
+        f32x4 z = zero4;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            f32x4 y = o[rt][d] * f0 + xo[((other * 4 + w4) * DT + d) * 64 + lane] * f1;
+            z += y * 0.0f;
+            y *= a.parts == 1 ? inv : unit;
+            if (!valid) continue;
+            if (a.parts == 1) *(f32x4 *)(a.out + row_at(r) * DH + 16 * d + 4 * g) = y;
+            else *(f32x4 *)(a.xo + at * DH + 16 * d + 4 * g) = y;
+        }
+        if (valid && a.parts > 1 && g == 0) {
+            a.xm[at] = mm;
+            a.xl[at] = ls;
+        }
+        bad = valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f);
+    }
+    // A masked position is in its tile's products with weight 0, which a V row
+    // that is not finite turns into NaN for the rows that do not see it: where
+    // an output is not finite, the block's rows are walked again one by one.
+    if (bad) odd = 1;
+    __syncthreads();
+    if (!odd) return;
+    constexpr int DL = RowState<DH>::DL;
+    for (int r = wid; r < nr; r += WP_NT / 64) {
+        const size_t qa = row_at(r) * DH + lane * DL;
+        const int p = a.pos0 + (r0 + r) / G;
+        RowState<DH> s;
+        s.m = -INFINITY;
+        s.l = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DL; d++) {
+            s.q[d] = a.q[qa + d];
+            s.o[d] = 0.0f;
+        }
+        for (int u = u0; u < u1; u++) {
+            const int t = tile(u), p0 = start(t), end = min(min(p0 + TP, limit(t)), p + 1);
+            row_walk<DH, KT>(s, (const KT *)a.k + base, (const KT *)a.v + base, p0, min(end, a.sinks));
+            row_walk<DH, KT>(s, (const KT *)a.k + base, (const KT *)a.v + base,
+                             max(max(p0, p + 1 - a.window), min(a.sinks, end)), end);
+        }
+        const size_t at = ((size_t)kvh * rows + r0 + r) * a.parts + part;
+#pragma unroll
+        for (int d = 0; d < DL; d++) {
+            if (a.parts == 1) a.out[qa + d] = s.o[d] / s.l;
+            else a.xo[at * DH + lane * DL + d] = s.o[d];
+        }
+        if (a.parts > 1 && lane == 0) {
+            a.xm[at] = s.m;
+            a.xl[at] = s.l;
+        }
+    }
+}
+
+// The parts of (query head, token) rows, a lane per four dimensions.
+template <int DH>
+__global__ __launch_bounds__(256) void k_prompt_parts(RowsArgs a)
+{
+    constexpr int LPR = DH / 4;
+    const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;   // of out
+    if (row >= (size_t)a.n * a.n_heads) return;
+    const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
+    const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
+    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
+        *m = a.xm + x0 + j;
+        *l = a.xl + x0 + j;
+        *x = a.xo + (x0 + j) * DH;
+    });
+    *(f32x4 *)(a.out + row * DH + 4 * d4) = o;
+}
+
+int launch_prompt_parts(const RowsArgs &a, hipStream_t s)
+{
+    const dim3 grid((unsigned)(((size_t)a.n * a.n_heads * a.d_head + 1023) / 1024)), block(256);
+#define MERGE(DH) hipLaunchKernelGGL(k_prompt_parts<DH>, grid, block, 0, s, a);
+    RW_BY_D_HEAD(a.d_head, MERGE)
+#undef MERGE
+    return 0;
+}
+
+bool wprompt_takes(int n, int n_heads, int n_kv, int d_head)
+{
+    return (d_head == 64 || d_head == 128) && (long)n * (n_heads / n_kv) >= 64;
+}
+
+// Parts of the positions: what the rounds of one work-group per CU and the
+// merge's traffic cost together, in steps of a pair of tiles (about a
+// microsecond).
+int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16)
+{
+    const int G = n_heads / n_kv, tp = kv_f16 ? 64 : WP_TS;
+    const long blocks = (long)n_kv * ceil_div((long)n * G, WP_ROWS);
+    const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + std::min(n, WP_ROWS / G + 1));
+    const long pairs = ceil_div(seen, 2 * tp) + 1;
+    int best = 1;
+    double least = 0;
+    for (int p = 1; p <= 16 && p <= pairs; p++) {
+        const double merge = p > 1 ? 4.0 + p * (double)n * n_heads * d_head * 8 / 4e6 : 0.0;
+        const double cost = (double)ceil_div(blocks * p, 256) * (ceil_div(pairs, p) + 2) + merge;
+        if (p == 1 || cost < least) {
+            best = p;
+            least = cost;
+        }
+    }
+    return best;
+}
+
+// Bytes of the split copy: the tiles, and their exponents behind them.
+size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window, int sinks)
+{
+    const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + n);
+    const size_t tiles = (size_t)n_kv * (ceil_div(seen, WP_TS) + 2);
+    return tiles * (WP_TS * d_head * 8 + 8);
+}
+
+template <int DH, bool F16>
+static int launch_dh(const RowsArgs &a, hipStream_t s)
+{
+    constexpr int LDS = 4 * (F16 ? 64 * DH * 4 : wp_tile_halves<DH>() * 2);
+    static LdsLimit limit;
+    const bool ok = limit.raise(current_device(), [] {
+        return hipFuncSetAttribute((const void *)k_prompt_rows<DH, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) ==
+               hipSuccess;
+    });
+    if (!ok) {
+        (void)hipGetLastError();
+        return -4;
+    }
+    int tiles = 0;
+    _Float16 *split = (_Float16 *)a.split;
+    int *exps = nullptr;
+    if constexpr (!F16) {
+        tiles = PromptTiles(a.pos0, a.window, a.sinks, WP_TS).count(a.pos0 + a.n - 1, WP_TS);
+        exps = (int *)(split + (size_t)a.n_kv * tiles * wp_tile_halves<DH>());
+        hipLaunchKernelGGL(k_prompt_split<DH>, dim3(tiles, a.n_kv), dim3(256), 0, s, a, split, exps, tiles);
+    }
+    const int blocks = ceil_div((long)a.n * (a.n_heads / a.n_kv), WP_ROWS);
+    hipLaunchKernelGGL((k_prompt_rows<DH, F16>), dim3(a.n_kv * blocks, a.parts), dim3(WP_NT), LDS, s, a, split, exps, tiles);
+    return 0;
+}
+
+int launch_wprompt(const RowsArgs &a0, hipStream_t s)
+{
+    RowsArgs a = a0;
+    a.parts = std::min(a.parts, wprompt_parts(a.n, a.n_heads, a.n_kv, a.d_head, a.max_ctx, a.window, a.sinks, a.kv_f16));
+    int rc;
+    if (a.kv_f16) rc = a.d_head == 128 ? launch_dh<128, true>(a, s) : launch_dh<64, true>(a, s);
+    else rc = a.d_head == 128 ? launch_dh<128, false>(a, s) : launch_dh<64, false>(a, s);
+    if (!rc && a.parts > 1) rc = launch_prompt_parts(a, s);
+    return rc ? rc : hipGetLastError() == hipSuccess ? 0 : -4;
+}

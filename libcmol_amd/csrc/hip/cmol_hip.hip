@@ -602,10 +602,11 @@ bool rows_shape(int n, int n_heads, int n_kv, int d_head, int max_ctx, int *rc)
     return true;
 }
 
-// Workspace of a plan: (m, l, o[d_head]) per partial result.
+// Workspace of a plan: the split copy, then (m, l, o[d_head]) per partial
+// result.
 size_t plan_bytes(const RowsPlan &p, int d_head)
 {
-    return align_up((p.pieces + p.cross) * (d_head + 2) * sizeof(float), ALIGN) + ALIGN;
+    return align_up(p.split, ALIGN) + align_up((p.pieces + p.cross) * (d_head + 2) * sizeof(float), ALIGN) + ALIGN;
 }
 
 size_t window_bytes(bool prompt, int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks,
@@ -659,7 +660,8 @@ bool rows_args(RowsArgs &a, cmolhip_ctx_t *c, int n, const float *q, const void 
     a.kv_f16 = kv_f16 != 0;
     a.bal = p.bal;
     a.parts = p.parts;
-    a.po = (float *)ws;
+    a.split = ws;
+    a.po = (float *)((uint8_t *)ws + align_up(p.split, ALIGN));
     a.xo = a.po + p.pieces * d_head;
     a.pm = a.xo + p.cross * d_head;
     a.pl = a.pm + p.pieces;

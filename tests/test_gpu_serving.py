@@ -184,6 +184,10 @@ PROMPT_CASES = [
     (8, 1, 32, 100, 60, 160, 33, 50), (8, 2, 256, 40, 30, 90, 25, 2), (32, 1, 64, 19, 100, 200, 64, 3),
     (20, 2, 128, 23, 9, 40, 2**31 - 1, 0), (6, 2, 64, 50, 10, 70, 8, 2**31 - 1), (15, 5, 64, 300, 250, 600, 120, 64),
     (3, 3, 128, 200, 0, 256, 100, 0), (5, 1, 64, 64, 64, 128, 32, 0),
+    # sinks of more than a tile, apart from the window, met by it and reaching into it; a window of everything
+    (16, 4, 128, 150, 900, 1100, 500, 70), (16, 4, 128, 260, 0, 300, 100, 70), (15, 5, 64, 333, 100, 500, 64, 300),
+    (16, 4, 128, 140, 150, 300, 100, 200), (8, 2, 64, 700, 0, 700, 5000, 0), (4, 1, 128, 129, 63, 256, 65, 64),
+    (2, 1, 64, 32, 0, 32, 1, 0), (2, 1, 128, 33, 31, 64, 33, 31),
 ]
 
 
@@ -224,6 +228,25 @@ def test_prompt_positions_that_are_not_finite(ctx, heads, kv, dh, f16):
             continue
         want, tol = reference(q[i].astype(np.float64), k.astype(np.float64), v.astype(np.float64), seen)
         close(got[i], want, tol, f"token {i}")
+
+
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("k_scale,v_scale", [(1e-6, 1e-6), (1e-3, 1e9), (1e-30, 1e-30), (1e3, 1.0), (1.0, 1e30)])
+def test_prompt_over_caches_of_any_range(ctx, dh, k_scale, v_scale):
+    """fp32 caches far from 1, each position's row times another power of ten
+    up to 10^4; the queries make up for K, so the scores are ordinary.  The
+    absolute term: a value of a tile of 32 positions is held to 2^-33 of the
+    tile's largest."""
+    heads, kv, n, pos0, max_ctx, window, sinks = 8, 2, 70, 100, 200, 90, 5
+    rng = np.random.default_rng(int(dh + np.log10(v_scale)))
+    q = (rng.standard_normal((n, heads, dh)) / k_scale / 1e3).astype(np.float32)
+    k = (rng.standard_normal((kv, max_ctx, dh)) * k_scale * 10 ** rng.uniform(0, 4, (kv, max_ctx, 1))).astype(np.float32)
+    v = (rng.standard_normal((kv, max_ctx, dh)) * v_scale * 10 ** rng.uniform(0, 4, (kv, max_ctx, 1))).astype(np.float32)
+    got = prompt_call(ctx, q, ctx.upload(k), ctx.upload(v), pos0, heads, kv, dh, max_ctx, 0, window, sinks)
+    for i in range(n):
+        seen = window_seen(pos0 + i + 1, max_ctx, window, sinks)
+        want, tol = reference(q[i].astype(np.float64), k.astype(np.float64), v.astype(np.float64), seen)
+        close(got[i] / v_scale, want / v_scale, tol / v_scale + 2.0**-33 * np.abs(v / v_scale).max(), f"token {i}")
 
 
 def test_prompt_tokens_equal_single_tokens(ctx):
