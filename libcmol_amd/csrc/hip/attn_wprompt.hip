@@ -3,16 +3,15 @@
 // through LDS.
 //
 // Rows of a kv head are (token, head of the group), token-major.  A work-group
-// of eight waves takes 128 of them and a part of the tiles of TP positions that
-// their tokens see between them; the waves of one half walk every second tile,
-// wave w4 of a half owns rows 32 w4 .. +31 (two tiles of 16), and the halves'
-// softmaxes and outputs meet at the end.  The next two tiles are copied into
-// LDS by direct-to-LDS loads while the present ones are used.
-//   fp16 cache (TP = 64): K pieces of 1 KiB in the operand's order (16 positions
+// of four waves takes 128 of them and a part of the tiles of 32 positions that
+// their tokens see between them; wave w owns rows 32 w .. +31 (two tiles of 16).
+// The next tile is copied into LDS by direct-to-LDS loads while the present one
+// is used.
+//   fp16 cache: K pieces of 1 KiB in the operand's order (16 positions
 //     x 32 dimensions, gathered by the loads' addresses), V rows as cached, their
 //     32-byte units XOR-swizzled by the row for the transposing reads
 //     (ds_read_b64_tr_b16) of the second product.
-//   fp32 cache (TP = 32): k_prompt_split lays the positions the prompt sees out
+//   fp32 cache: k_prompt_split lays the positions the prompt sees out
 //     once per call as f16 pairs (x = hi + lo), both operands in their order.
 //     A tile is scaled by a power of two that puts its largest |K| (|V|) into
 //     [2^9, 2^10), so hi and lo are normal f16 numbers whatever the cache's
@@ -26,7 +25,7 @@
 #include "attn_rows.h"
 #include "lds_limit.h"
 
-constexpr int WP_NT = 512, WP_ROWS = 128, WP_TS = 32;   // threads, rows, positions of a split tile
+constexpr int WP_NT = 256, WP_ROWS = 128, WP_TP = 32;   // threads, rows, positions of a tile
 
 // Tiles of TP positions that a prompt's tokens see: `ns` of sinks, then the
 // run from lo (where the sinks reach into it, one run from 0).
@@ -42,9 +41,9 @@ struct PromptTiles {
     __host__ __device__ int count(int last, int tp) const { return ns + (last + tp - lo) / tp; }
 };
 
-// A split tile: K hi and lo pieces, V hi and lo pieces, WP_TS positions.
+// A split tile: K hi and lo pieces, V hi and lo pieces, WP_TP positions.
 template <int DH>
-constexpr int wp_tile_halves() { return WP_TS * DH * 4; }
+constexpr int wp_tile_halves() { return WP_TP * DH * 4; }
 
 template <int DH>
 __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst, int *exps, int tiles)
@@ -53,9 +52,9 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
     constexpr int KS = DH / 32, DT = DH / 16, NK = 2 * KS * 64 / 256, NV = DT * 64 / 256, TH = wp_tile_halves<DH>();
     __shared__ float top[2][4];
     const int tile = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
-    const PromptTiles pt(a.pos0, a.window, a.sinks, WP_TS);
-    const int p0 = tile < pt.ns ? tile * WP_TS : pt.lo + (tile - pt.ns) * WP_TS;
-    const int cnt = min(WP_TS, (tile < pt.ns ? pt.s : a.pos0 + a.n) - p0);
+    const PromptTiles pt(a.pos0, a.window, a.sinks, WP_TP);
+    const int p0 = tile < pt.ns ? tile * WP_TP : pt.lo + (tile - pt.ns) * WP_TP;
+    const int cnt = min(WP_TP, (tile < pt.ns ? pt.s : a.pos0 + a.n) - p0);
     const size_t base = ((size_t)kvh * a.max_ctx + p0) * DH;
     const float *kb = (const float *)a.k + base, *vb = (const float *)a.v + base;
     dst += ((size_t)kvh * tiles + tile) * TH;
@@ -120,24 +119,26 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
     }
 }
 
+// LDS of a work-group: two stages of K and V.
+template <int DH, bool F16>
+constexpr int wp_lds() { return 2 * (F16 ? WP_TP * DH * 4 : wp_tile_halves<DH>() * 2); }
+
 template <int DH, bool F16>
 __global__ __launch_bounds__(WP_NT) __attribute__((amdgpu_waves_per_eu(2)))
 void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles)
 {
 #pragma clang fp contract(off)
     typedef typename std::conditional<F16, _Float16, float>::type KT;
-    constexpr int TP = F16 ? 64 : WP_TS, CT = TP / 16, RT = 2;
+    constexpr int TP = WP_TP, CT = TP / 16, RT = 2;
     constexpr int KS = DH / 32, DT = DH / 16;
     constexpr int KB = F16 ? TP * DH * 2 : wp_tile_halves<DH>();   // K bytes of a tile (V: as many)
-    constexpr int TILE = 2 * KB;
     constexpr int RPP = 1024 / (2 * DH);              // fp16: V rows per 1 KiB piece
     constexpr int VPW = TP / RPP / 4;                 // fp16: V pieces per wave
-    constexpr int PIECES = TILE / 1024 / 4;           // fp32: pieces per wave
-    extern __shared__ __attribute__((aligned(256))) uint8_t smem_w[];   // [stage][half][TILE]
+    extern __shared__ __attribute__((aligned(256))) uint8_t smem_w[];   // K [stage][KB], V the same
     __shared__ int odd;
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
-    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), half = wid >> 2, w4 = wid & 3;
+    const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.n_heads / a.n_kv, rows = a.n * G;
     const int blocks = gridDim.x / a.n_kv;
     // the blocks of the longest lines first
@@ -149,7 +150,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     const int lo = max(first + 1 - a.window, 0);
     const int na = pt.s || !a.sinks ? pt.ns : (min(a.sinks, lo) + TP - 1) / TP;
     const int nb = max(pt.ns + (lo - pt.lo) / TP, na), ne = pt.count(last, TP);
-    const int T = na + ne - nb, R = ((T + a.parts - 1) / a.parts + 1) & ~1;   // (pairs of tiles)
+    const int T = na + ne - nb, R = (T + a.parts - 1) / a.parts;
     const int u0 = min(part * R, T), u1 = min(u0 + R, T);
     auto tile = [&](int u) { return u < na ? u : u - na + nb; };
     auto start = [&](int t) { return t < pt.ns ? t * TP : pt.lo + (t - pt.ns) * TP; };
@@ -159,50 +160,73 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     const uint8_t *kb = (const uint8_t *)uniform_ptr((const KT *)a.k + base);
     const uint8_t *vbp = (const uint8_t *)uniform_ptr((const KT *)a.v + base);
     const uint8_t *sb = (const uint8_t *)uniform_ptr(split + (size_t)kvh * tiles * wp_tile_halves<DH>());
-    const int *ex = uniform_ptr(exps + (size_t)kvh * tiles * 2);
+    typedef const __attribute__((address_space(4))) int cint;   // (scalar loads)
+    cint *ex = (cint *)uniform_ptr(exps + (size_t)kvh * tiles * 2);
     const int vrow = lane / (DH / 8), vch = lane % (DH / 8);
-    auto issue = [&](int st, int u) {
-        uint8_t *dst = smem_w + (st * 2 + half) * TILE;
+    uint8_t *const kl_ = smem_w, *const vl_ = smem_w + 2 * KB;
+    auto issue_k = [&](int st, int u) {
+        uint8_t *dst = kl_ + st * KB;
         const int t = tile(u);
         if constexpr (F16) {
             const int p0 = start(t), cnt = limit(t) - p0;   // (past it: its last position again)
-            const uint8_t *ks = kb + (size_t)p0 * (2 * DH), *vs = vbp + (size_t)p0 * (2 * DH);
-            const uint32_t kp = (uint32_t)min(16 * w4 + col, cnt - 1) * (2 * DH) + 16 * g;
+            const uint8_t *ks = kb + (size_t)p0 * (2 * DH);
 #pragma unroll
-            for (int s = 0; s < KS; s++)
-                __builtin_amdgcn_global_load_lds((const gvoid_t *)(ks + kp + 64 * s), (lvoid_t *)(dst + (w4 * KS + s) * 1024),
-                                                 16, 0, 0);
-#pragma unroll
-            for (int i = 0; i < VPW; i++) {
-                const int r = (w4 * VPW + i) * RPP + vrow;   // row of the tile
-                const int f = DH == 128 ? r & 7 : (r >> 1) & 3;
-                const uint32_t vp = (uint32_t)min(r, cnt - 1) * (2 * DH) + 32 * ((vch >> 1) ^ f) + 16 * (vch & 1);
-                __builtin_amdgcn_global_load_lds((const gvoid_t *)(vs + vp),
-                                                 (lvoid_t *)(dst + KB + (w4 * VPW + i) * 1024), 16, 0, 0);
+            for (int i = 0; i < CT * KS / 4; i++) {
+                const int pc = wid * (CT * KS / 4) + i;   // 16 positions x 32 dimensions
+                const uint32_t kp = (uint32_t)min(16 * (pc / KS) + col, cnt - 1) * (2 * DH) + 64 * (pc % KS) + 16 * g;
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(ks + kp), (lvoid_t *)(dst + pc * 1024), 16, 0, 0);
             }
         } else {
-            const uint8_t *src = sb + (size_t)t * TILE;
+            const uint8_t *src = sb + (size_t)t * (2 * KB);
 #pragma unroll
-            for (int i = 0; i < PIECES; i++) {
-                const int pc = w4 * PIECES + i;
-                __builtin_amdgcn_global_load_lds((const gvoid_t *)(src + pc * 1024 + lane * 16),
-                                                 (lvoid_t *)(dst + pc * 1024), 16, 0, 0);
+            for (int i = 0; i < KB / 4096; i++) {
+                const int pc = wid * (KB / 4096) + i;
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(src + pc * 1024 + lane * 16), (lvoid_t *)(dst + pc * 1024),
+                                                 16, 0, 0);
             }
         }
     };
-    if (u0 + half < u1) issue(0, u0 + half);
+    auto issue_v = [&](int st, int u) {
+        uint8_t *dst = vl_ + st * KB;
+        const int t = tile(u);
+        if constexpr (F16) {
+            const int p0 = start(t), cnt = limit(t) - p0;
+            const uint8_t *vs = vbp + (size_t)p0 * (2 * DH);
+#pragma unroll
+            for (int i = 0; i < VPW; i++) {
+                const int r = (wid * VPW + i) * RPP + vrow;   // row of the tile
+                const int f = DH == 128 ? r & 7 : (r >> 1) & 3;
+                const uint32_t vp = (uint32_t)min(r, cnt - 1) * (2 * DH) + 32 * ((vch >> 1) ^ f) + 16 * (vch & 1);
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(vs + vp), (lvoid_t *)(dst + (wid * VPW + i) * 1024), 16, 0, 0);
+            }
+        } else {
+            const uint8_t *src = sb + (size_t)t * (2 * KB) + KB;
+#pragma unroll
+            for (int i = 0; i < KB / 4096; i++) {
+                const int pc = wid * (KB / 4096) + i;
+                __builtin_amdgcn_global_load_lds((const gvoid_t *)(src + pc * 1024 + lane * 16), (lvoid_t *)(dst + pc * 1024),
+                                                 16, 0, 0);
+            }
+        }
+    };
+    // K runs a tile ahead of V: the next tile's scores are computed beside the
+    // present one's weights
+    if (u0 < u1) {
+        issue_k(0, u0);
+        issue_v(0, u0);
+    }
 
     auto row_at = [&](int r) {   // of q and out
         r = min(r0 + r, rows - 1);
         return (size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G;
     };
-    // query operands of rows 32 w4 + 16 rt + col: the row's largest into [2^9, 2^10)
+    // query operands of rows 32 wid + 16 rt + col: the row's largest into [2^9, 2^10)
     f16x8 qh[RT][KS], ql[RT][KS];
     float c2[RT];
     int pos[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int r = 32 * w4 + 16 * rt + col;
+        const int r = 32 * wid + 16 * rt + col;
         pos[rt] = a.pos0 + min(r0 + r, rows - 1) / G;
         const float *q = a.q + row_at(r) * DH + 8 * g;
         float x[KS][8], top = 0.0f;
@@ -253,52 +277,89 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     const int vr = 4 * g + (col >> 2);
     const uint32_t vaddr = (uint32_t)(vr * (2 * DH) + 32 * (DH == 128 ? vr & 7 : (vr >> 1) & 3) + 8 * (col & 3));
 
-    int st = 0;
-    for (int uu = u0; uu < u1; uu += 2, st ^= 1) {
-        const int u = uu + half;
-        // the tiles have landed and every wave is done with the other stage
+    // operand pieces: q-th of a K tile (c = q / KS, s = q % KS), d-th of a V tile
+    // (dimension tile d)
+    static_assert(CT == 2, "two groups of 16 positions");
+    constexpr int NP = F16 ? 1 : 2;
+    auto read_k = [&](int st, int q, f16x8 (&x)[NP]) {
+        const uint8_t *src = kl_ + st * KB + q * NP * 1024 + lane * 16;
+#pragma unroll
+        for (int i = 0; i < NP; i++) x[i] = *(const f16x8 *)(src + i * 1024);
+    };
+    auto read_v = [&](int st, int d, f16x8 (&x)[NP]) {
+        const uint8_t *src = vl_ + st * KB;
+        if constexpr (F16) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4 ls16x4;
+            src += vaddr ^ (32u * d);
+            const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)src);
+            const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)(src + 16 * (2 * DH)));
+            x[0] = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+#pragma unroll
+            for (int i = 0; i < NP; i++) x[i] = *(const f16x8 *)(src + (d * NP + i) * 1024 + lane * 16);
+        }
+    };
+    // Products of two pieces with the row tiles' operands into y[piece][rt], those
+    // with a low part first; consecutive ones on different sums.
+    auto products = [&](const f16x8 (&x)[2][NP], const f16x8 *(&hi)[RT], const f16x8 *(&lo)[RT], f32x4 *(&y)[2][RT]) {
+#pragma unroll
+        for (int t = F16 ? 1 : 0; t < 3; t++)
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+                    *y[i][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i][t == 0 ? NP - 1 : 0], t == 1 ? *lo[rt] : *hi[rt],
+                                                                       *y[i][rt], 0, 0, 0);
+    };
+    auto score_step = [&](const f16x8 (&x)[2][NP], int s, f32x4 (&y)[RT][CT]) {   // k-step s of both c
+        const f16x8 *hi[RT], *lo[RT];
+        f32x4 *at[2][RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            hi[rt] = &qh[rt][s];
+            lo[rt] = &ql[rt][s];
+#pragma unroll
+            for (int c = 0; c < CT; c++) {
+                at[c][rt] = &y[rt][c];
+                if (s == 0) y[rt][c] = zero4;
+            }
+        }
+        products(x, hi, lo, at);
+    };
+    // sc[rt][c][i]: score of the tile's position 16c + 4g + i and row col
+    f32x4 sc[RT][CT];
+    __builtin_amdgcn_s_waitcnt(WAITCNT_VM_LGKM0(0));
+    __syncthreads();
+    if (u0 + 1 < u1) issue_k(1, u0 + 1);
+    int ek = 0, ev = 0;   // exponents of the tile
+    if (u0 < u1) {
+#pragma unroll
+        for (int q = 0; q < KS; q++) {
+            f16x8 k[2][NP];
+            read_k(0, q, k[0]);
+            read_k(0, KS + q, k[1]);
+            score_step(k, q, sc);
+        }
+        if constexpr (!F16) {
+            ek = ex[2 * tile(u0)];
+            ev = ex[2 * tile(u0) + 1];
+        }
+    }
+    for (int u = u0, st = 0; u < u1; u++, st ^= 1) {
+        // K u + 1 and V u have landed, every wave is done with K u and V u - 1
         __builtin_amdgcn_s_waitcnt(WAITCNT_VM_LGKM0(0));
         __syncthreads();
-        if (u + 2 < u1) issue(st ^ 1, u + 2);
-        if (u >= u1) continue;   // (the last pair may be one tile)
-        const uint8_t *ks_ = smem_w + (st * 2 + half) * TILE, *vs_ = ks_ + KB;
+        if (u + 2 < u1) issue_k(st, u + 2);
+        if (u + 1 < u1) issue_v(st ^ 1, u + 1);
         const int t = tile(u), p0 = start(t), cnt = limit(t) - p0;
         float kf = 1.0f, vf = 1.0f;
         if constexpr (!F16) {
-            kf = ldexpf(1.0f, ex[2 * t]);
-            vf = ldexpf(1.0f, ex[2 * t + 1] - ve);
-        }
-        // ---- scores: sc[rt][c][i] = position p0 + 16c + 4g + i of row col
-        float sc[RT][CT][4];
-#pragma unroll
-        for (int c = 0; c < CT; c++) {
-            f32x4 s1[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) s1[rt] = zero4;
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                if constexpr (F16) {
-                    const f16x8 k = *(const f16x8 *)(ks_ + (c * KS + s) * 1024 + lane * 16);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][s], s1[rt], 0, 0, 0);
-                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][s], s1[rt], 0, 0, 0);
-                    }
-                } else {
-                    const f16x8 kh = *(const f16x8 *)(ks_ + (c * KS + s) * 2048 + lane * 16);
-                    const f16x8 kl = *(const f16x8 *)(ks_ + (c * KS + s) * 2048 + 1024 + lane * 16);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, qh[rt][s], s1[rt], 0, 0, 0);
-                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[rt][s], s1[rt], 0, 0, 0);
-                        s1[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[rt][s], s1[rt], 0, 0, 0);
-                    }
-                }
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) sc[rt][c][i] = s1[rt][i];
+            kf = ldexpf(1.0f, ek);
+            vf = ldexpf(1.0f, ev - ve);
+            const int tn = tile(min(u + 1, u1 - 1));   // (its exponents in time)
+            ek = ex[2 * tn];
+            ev = ex[2 * tn + 1];
         }
         const int top = p0 + TP - 1;
         if (top > first || cnt < TP || (top >= a.sinks && p0 <= last - a.window)) {   // uniform
@@ -312,22 +373,27 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
                         if (at >= cnt || p > pos[rt] || (p >= a.sinks && p <= pos[rt] - a.window)) sc[rt][c][i] = -INFINITY;
                     }
         }
-        // ---- online softmax
-        f16x8 ph[RT][CT / 2], pl[RT][CT / 2];
+        // ---- online softmax: the reference
+        float f[RT], mx[RT];
+        bool up = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             // (above 0: a masked score times it stays -inf)
-            const float f = F16 ? c2[rt] : fmaxf(c2[rt] * kf, 1e-37f);
-            float mx = sc[rt][0][0];
+            f[rt] = F16 ? c2[rt] : fmaxf(c2[rt] * kf, 1e-37f);
+            mx[rt] = sc[rt][0][0];
 #pragma unroll
             for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[rt][c][i]);
-            mx *= f;
-            if (__ballot(mx > m[rt] + RW_LAZY)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(m[rt], mx);
+                for (int i = 0; i < 4; i++) mx[rt] = fmaxf(mx[rt], sc[rt][c][i]);
+            mx[rt] *= f[rt];
+            up |= mx[rt] > m[rt] + RW_LAZY;
+        }
+        if (__ballot(up)) {   // (one branch for both row tiles: what follows is one block to schedule)
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 16, 64));
+                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 32, 64));
+                const float mn = fmaxf(m[rt], mx[rt]);
                 const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn;
                 const float al = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - mk[rt]);
                 m[rt] = mn;
@@ -336,109 +402,105 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
 #pragma unroll
                 for (int d = 0; d < DT; d++) o[rt][d] *= al;
             }
-            float ls = 0.0f;
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i += 2) {
-                    float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], f, mk[rt]));
-                    float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], f, mk[rt]));
-                    ls += e0 + e1;
-                    if constexpr (!F16) {
-                        e0 *= vf;
-                        e1 *= vf;
-                    }
-                    const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0, e1));
-                    const f16x2 lw =
-                        __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0 - (float)hi[0], e1 - (float)hi[1]));
-                    ph[rt][c >> 1][4 * (c & 1) + i] = hi[0];
-                    ph[rt][c >> 1][4 * (c & 1) + i + 1] = hi[1];
-                    pl[rt][c >> 1][4 * (c & 1) + i] = lw[0];
-                    pl[rt][c >> 1][4 * (c & 1) + i + 1] = lw[1];
-                }
-            l[rt] += ls;
         }
-        // ---- O^T += V^T P^T: k-step k covers positions 32k + 4g .. +3 and 32k + 16 + 4g .. +3
-#pragma unroll
-        for (int k = 0; k < CT / 2; k++) {
-#pragma unroll
-            for (int d = 0; d < DT; d++) {
-                if constexpr (F16) {
-                    typedef short s16x4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s16x4 ls16x4;
-                    const uint8_t *src = vs_ + 32 * k * (2 * DH) + (vaddr ^ (32u * d));
-                    const s16x4 lo4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)src);
-                    const s16x4 hi4 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls16x4 *)(src + 16 * (2 * DH)));
-                    const f16x8 v = __builtin_bit_cast(f16x8, __builtin_shufflevector(lo4, hi4, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[rt][k], o[rt][d], 0, 0, 0);
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[rt][k], o[rt][d], 0, 0, 0);
-                    }
-                } else {
-                    const f16x8 vh = *(const f16x8 *)(vs_ + d * 2048 + lane * 16);
-                    const f16x8 vl = *(const f16x8 *)(vs_ + d * 2048 + 1024 + lane * 16);
-#pragma unroll
-                    for (int rt = 0; rt < RT; rt++) {
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, ph[rt][k], o[rt][d], 0, 0, 0);
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, pl[rt][k], o[rt][d], 0, 0, 0);
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, ph[rt][k], o[rt][d], 0, 0, 0);
-                    }
-                }
+        // ---- the weights (P, in two parts) between the next tile's scores, then
+        // O^T += V^T P^T.  The order is fixed: a step's operand pieces are read
+        // during the one before, and its products run beside its share of the weights'
+        // instructions.  (A K stage past the last tile holds an old one: not used.)
+        f32x4 sn[RT][CT];
+        f16x8 kr[2][2][NP], ph[RT], pl[RT];
+        float ls[RT];
+        constexpr int PAIRS = RT * CT * 2;
+        auto weights = [&](int x) {   // scores 2x, 2x + 1 of (rt, c, i)
+            const int rt = x / (CT * 2), c = x / 2 % CT, i = x % 2 * 2;
+            float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], f[rt], mk[rt]));
+            float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], f[rt], mk[rt]));
+            ls[rt] += e0 + e1;
+            if constexpr (!F16) {
+                e0 *= vf;
+                e1 *= vf;
             }
+            const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0, e1));
+            const f16x2 lw = __builtin_bit_cast(
+                f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], -1.0f, e0), fmaf((float)hi[1], -1.0f, e1)));
+            ph[rt][4 * c + i] = hi[0];
+            ph[rt][4 * c + i + 1] = hi[1];
+            pl[rt][4 * c + i] = lw[0];
+            pl[rt][4 * c + i + 1] = lw[1];
+        };
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) ls[rt] = 0.0f;
+        read_k(st ^ 1, 0, kr[0][0]);
+        read_k(st ^ 1, KS, kr[0][1]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < KS; q++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                if (q + 1 < KS) read_k(st ^ 1, i * KS + q + 1, kr[(q + 1) & 1][i]);
+                else read_v(st, i, kr[(q + 1) & 1][i]);
+            }
+            score_step(kr[q & 1], q, sn);
+#pragma unroll
+            for (int x = q * PAIRS / KS; x < (q + 1) * PAIRS / KS; x++) weights(x);
+            __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) l[rt] += ls[rt];
+#pragma unroll
+        for (int d = 0; d < DT; d += 2) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (d + 2 < DT) read_v(st, d + 2 + i, kr[(KS + d / 2 + 1) & 1][i]);
+            const f16x8 *hi[RT], *lo[RT];
+            f32x4 *at[2][RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                hi[rt] = &ph[rt];
+                lo[rt] = &pl[rt];
+                at[0][rt] = &o[rt][d];
+                at[1][rt] = &o[rt][d + 1];
+            }
+            products(kr[(KS + d / 2) & 1], hi, lo, at);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int c = 0; c < CT; c++) sc[rt][c] = sn[rt][c];
     }
 
-    // ---- the halves meet: each finishes one of the two row tiles
-    if (tid == 0) odd = 0;
-    f32x4 *xo = (f32x4 *)smem_w;                              // [half][wave][DT][lane]
-    float *xm = (float *)(smem_w + 8 * DT * 64 * 16);         // [half][wave][lane] m, then l
-    __syncthreads();
-    const int mine = half, other = half ^ 1;                  // row tiles kept and handed over
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) m[rt] = m[rt] == -INFINITY ? -INFINITY : -mk[rt];   // of the weights as they are
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        if (rt == mine) continue;
-#pragma unroll
-        for (int d = 0; d < DT; d++) xo[((half * 4 + w4) * DT + d) * 64 + lane] = o[rt][d];
-        xm[(half * 4 + w4) * 64 + lane] = m[rt];
-        xm[512 + (half * 4 + w4) * 64 + lane] = l[rt];
-    }
-    __syncthreads();
+    // ---- outputs: lane (col, g) holds dimensions 16d + 4g + i of row col
     bool bad = false;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        if (rt != mine) continue;
-        const int x = (other * 4 + w4) * 64 + lane;
-        const float m1 = xm[x], mm = fmaxf(m[rt], m1), ref = mm == -INFINITY ? 0.0f : mm;
-        const float f0 = __builtin_amdgcn_exp2f(m[rt] - ref), f1 = __builtin_amdgcn_exp2f(m1 - ref);
-        float ls = l[rt] * f0 + xm[512 + x] * f1;
+        float ls = l[rt];
         ls += __shfl_xor(ls, 16, 64);
         ls += __shfl_xor(ls, 32, 64);
-        const int r = 32 * w4 + 16 * rt + col;
+        const int r = 32 * wid + 16 * rt + col;
         const bool valid = r < nr;
         const float unit = ldexpf(1.0f, ve), inv = unit / ls;
         const size_t at = ((size_t)kvh * rows + min(r0 + r, rows - 1)) * a.parts + part;
         f32x4 z = zero4;
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-            f32x4 y = o[rt][d] * f0 + xo[((other * 4 + w4) * DT + d) * 64 + lane] * f1;
+            const f32x4 y = o[rt][d] * (a.parts == 1 ? inv : unit);
             z += y * 0.0f;
-            y *= a.parts == 1 ? inv : unit;
             if (!valid) continue;
             if (a.parts == 1) *(f32x4 *)(a.out + row_at(r) * DH + 16 * d + 4 * g) = y;
             else *(f32x4 *)(a.xo + at * DH + 16 * d + 4 * g) = y;
         }
         if (valid && a.parts > 1 && g == 0) {
-            a.xm[at] = mm;
+            a.xm[at] = m[rt] == -INFINITY ? -INFINITY : -mk[rt];   // of the weights as they are
             a.xl[at] = ls;
         }
-        bad = valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f);
+        bad |= valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f);
     }
     // A masked position is in its tile's products with weight 0, which a V row
     // that is not finite turns into NaN for the rows that do not see it: where
     // an output is not finite, the block's rows are walked again one by one.
+    if (tid == 0) odd = 0;
+    __syncthreads();
     if (bad) odd = 1;
     __syncthreads();
     if (!odd) return;
@@ -504,20 +566,21 @@ bool wprompt_takes(int n, int n_heads, int n_kv, int d_head)
     return (d_head == 64 || d_head == 128) && (long)n * (n_heads / n_kv) >= 64;
 }
 
-// Parts of the positions: what the rounds of one work-group per CU and the
-// merge's traffic cost together, in steps of a pair of tiles (about a
-// microsecond).
+// Parts of the positions: what the rounds of two work-groups per CU and the
+// merge's traffic cost together, in microseconds (a tile and the start of a
+// work-group as they take at two per CU).
 int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16)
 {
-    const int G = n_heads / n_kv, tp = kv_f16 ? 64 : WP_TS;
+    const int G = n_heads / n_kv;
     const long blocks = (long)n_kv * ceil_div((long)n * G, WP_ROWS);
     const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + std::min(n, WP_ROWS / G + 1));
-    const long pairs = ceil_div(seen, 2 * tp) + 1;
+    const long tiles = ceil_div(seen, WP_TP) + 1;
+    const double step = (kv_f16 ? 1.4 : 2.0) * d_head / 128;
     int best = 1;
     double least = 0;
-    for (int p = 1; p <= 16 && p <= pairs; p++) {
-        const double merge = p > 1 ? 4.0 + p * (double)n * n_heads * d_head * 8 / 4e6 : 0.0;
-        const double cost = (double)ceil_div(blocks * p, 256) * (ceil_div(pairs, p) + 2) + merge;
+    for (int p = 1; p <= 16 && p <= tiles; p++) {
+        const double merge = p > 1 ? 4.0 + p * (double)n * n_heads * d_head * 8 / 5e6 : 0.0;
+        const double cost = ceil_div(blocks * p, RW_WGS) * (ceil_div(tiles, p) * step + 8.0) + merge;
         if (p == 1 || cost < least) {
             best = p;
             least = cost;
@@ -530,14 +593,14 @@ int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int win
 size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window, int sinks)
 {
     const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + n);
-    const size_t tiles = (size_t)n_kv * (ceil_div(seen, WP_TS) + 2);
-    return tiles * (WP_TS * d_head * 8 + 8);
+    const size_t tiles = (size_t)n_kv * (ceil_div(seen, WP_TP) + 2);
+    return tiles * (WP_TP * d_head * 8 + 8);
 }
 
 template <int DH, bool F16>
 static int launch_dh(const RowsArgs &a, hipStream_t s)
 {
-    constexpr int LDS = 4 * (F16 ? 64 * DH * 4 : wp_tile_halves<DH>() * 2);
+    constexpr int LDS = wp_lds<DH, F16>();
     static LdsLimit limit;
     const bool ok = limit.raise(current_device(), [] {
         return hipFuncSetAttribute((const void *)k_prompt_rows<DH, F16>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) ==
@@ -551,7 +614,7 @@ static int launch_dh(const RowsArgs &a, hipStream_t s)
     _Float16 *split = (_Float16 *)a.split;
     int *exps = nullptr;
     if constexpr (!F16) {
-        tiles = PromptTiles(a.pos0, a.window, a.sinks, WP_TS).count(a.pos0 + a.n - 1, WP_TS);
+        tiles = PromptTiles(a.pos0, a.window, a.sinks, WP_TP).count(a.pos0 + a.n - 1, WP_TP);
         exps = (int *)(split + (size_t)a.n_kv * tiles * wp_tile_halves<DH>());
         hipLaunchKernelGGL(k_prompt_split<DH>, dim3(tiles, a.n_kv), dim3(256), 0, s, a, split, exps, tiles);
     }
