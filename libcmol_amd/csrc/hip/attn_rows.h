@@ -9,16 +9,18 @@
 // there are none.  Every sum and softmax statistic is fp32.
 //
 // One walk serves all of them (rows_walk): a wave holds RT tiles of 16 query
-// rows of one kv head and takes tiles of 32 cached positions, straight from
-// the cache into the matrix instructions' operand registers; nothing is staged
-// in LDS and the waves of a work-group, on different tiles, meet only at the
-// end of their range (rows_finish).
+// rows of one kv head and takes tiles of TP cached positions (32 over fp16, 16
+// over fp32: the same bytes), straight from the cache into the matrix
+// instructions' operand registers; nothing is staged in LDS and the waves of a
+// work-group, on different tiles, meet only at the end of their range
+// (rows_finish).
 //   * scores transposed, S^T = K Q^T: the A operand's rows are 16 positions
 //     (16-byte pieces of the K rows as cached), the B operand's columns the
-//     query rows, so lane (col, g) holds positions 4g .. 4g+3 of row `col`;
+//     query rows, so lane (col, g) holds positions 4g .. 4g+3 of row `col` (of each
+//     16);
 //   * O^T += V^T P^T: the scores' layout is the B operand's as it is (k index
 //     of lane group g = positions 4g .. 4g+3, and 16 more of the tile's second
-//     half), and a lane's A operand for output tile e is dimension VD col + e of
+//     16, over fp16), and a lane's A operand for output tile e is dimension VD col + e of
 //     those positions, VD = d_head / 16: a lane loads VD neighbouring dimensions
 //     of its positions' V rows, 16 lanes a whole row, and for fp16 pairs of rows
 //     are interleaved with one v_perm_b32 per two values;
@@ -26,8 +28,8 @@
 //     than RW_LAZY (log2 units; a wave vote), so most tiles need no cross-lane
 //     step; weights are 2^(t c2 + mk), c2 = log2(e) / sqrt(d_head).
 // fp16 caches: 16x16x32 f16 products, exact, with fp32 sums.  The query is
-// scaled by a power of two per row into [1, 2) and split into two f16 parts (22
-// bits); a weight, scaled by 2^RW_SCALE, into two f16 parts whose products
+// scaled by a power of two per row into [2^9, 2^10) and split into two f16 parts
+// (22 bits, 2^-33 of the row's largest below) whose products share a sum; a weight, scaled by 2^RW_SCALE, into two f16 parts whose products
 // share an accumulator (22 bits of a weight down to 2^-16 of the largest, an
 // absolute 2^-36 of it below).  fp32 caches: 16x16x4 f32 products throughout.
 #pragma once
@@ -35,8 +37,7 @@
 
 #include <algorithm>
 
-constexpr int RW_TP = 32;            // positions per tile
-constexpr int RW_NW = 4;             // waves per work-group
+template <typename KT> constexpr int rw_tp() { return sizeof(KT) == 2 ? 32 : 16; }   // positions per tile
 constexpr int RW_PAD = 2;            // tiles that stand for the start of an item's piece
 constexpr float RW_LAZY = 2.0f;      // log2: weights stay below 2^(RW_SCALE + 2)
 constexpr float RW_SCALE = 12.0f;
@@ -66,44 +67,43 @@ struct RowsArgs {
 
 // Tiles of two runs of positions, [0, s) and [lo, hi): the first ns tiles
 // cover the first, the rest the second.
+template <int TP>
 struct RowsLine {
     int s, lo, hi, ns;
-    __device__ __forceinline__ int tiles() const { return ns + (hi - lo + RW_TP - 1) / RW_TP; }
+    __device__ __forceinline__ int tiles() const { return ns + (hi - lo + TP - 1) / TP; }
     // first position and number of positions of tile u
     __device__ __forceinline__ void tile(int u, int *p0, int *cnt) const
     {
-        *p0 = u < ns ? u * RW_TP : lo + (u - ns) * RW_TP;
-        *cnt = min(RW_TP, (u < ns ? s : hi) - *p0);
+        *p0 = u < ns ? u * TP : lo + (u - ns) * TP;
+        *cnt = min(TP, (u < ns ? s : hi) - *p0);
     }
 };
 
 // Positions that tokens at first .. last see between them.
-__device__ __forceinline__ RowsLine rows_line(int first, int last, int window, int sinks)
+template <int TP>
+__device__ __forceinline__ RowsLine<TP> rows_line(int first, int last, int window, int sinks)
 {
-    RowsLine l;
+    RowsLine<TP> l;
     l.hi = last + 1;
     l.lo = max(first + 1 - window, 0);
     l.s = min(sinks, l.lo);
-    l.ns = (l.s + RW_TP - 1) / RW_TP;
+    l.ns = (l.s + TP - 1) / TP;
     return l;
 }
 
-// Positions of item i's cache up to its own (0: it sees nothing there), and
-// that cache.
-__device__ __forceinline__ int rows_item(const RowsArgs &a, int i, size_t *base)
+// Item i: positions of its cache up to its own (0: it sees nothing there), and
+// which cache.
+__device__ __forceinline__ int rows_item(const RowsArgs &a, int i, int *slot)
 {
-    const int slot = a.slots ? a.slots[i] : i;
     const int L = a.seqlen[i];
-    *base = slot < 0 ? 0 : (size_t)slot * a.slot_stride;
-    return slot < 0 ? 0 : max(min(L, a.max_ctx), 0);
+    *slot = a.slots ? a.slots[i] : i;
+    return *slot < 0 ? 0 : max(min(L, a.max_ctx), 0);
 }
 
-__device__ __forceinline__ unsigned rows_tiles(const RowsArgs &a, int i)
+template <int TP>
+__device__ __forceinline__ unsigned rows_tiles(const RowsArgs &a, int L)
 {
-    if (i >= a.n) return 0;
-    size_t base;
-    const int L = rows_item(a, i, &base);
-    return L > 0 ? rows_line(L - 1, L - 1, a.window, a.sinks).tiles() : 0;
+    return L > 0 ? rows_line<TP>(L - 1, L - 1, a.window, a.sinks).tiles() : 0;
 }
 
 // Balanced ranges.  The items' tiles are laid end to end on one line, each
@@ -130,54 +130,93 @@ __device__ __forceinline__ unsigned wave_scan_u(unsigned v)   // inclusive
 }
 constexpr unsigned RW_RMIN = 4;   // tiles per range at least: one per wave
 
-// Range length; t0: this lane's item's tiles among the first 64.
-__device__ __forceinline__ unsigned rows_range(const RowsArgs &a, unsigned t0)
-{
-    const int lane = threadIdx.x & 63;
-    unsigned t = lane < a.n ? t0 + RW_PAD : 0;
-    for (int b = 64; b < a.n; b += 64) t += b + lane < a.n ? rows_tiles(a, b + lane) + RW_PAD : 0;
-    const unsigned line = wave_sum_u(t);
-    return max(RW_RMIN, (line + a.bal - 1) / a.bal);
-}
+// A lane's item among the first 64, and the range length (every wave works
+// them out, with no barrier).
+template <int TP>
+struct RowsSpread {
+    int L, slot;
+    unsigned T, R;
+    __device__ __forceinline__ explicit RowsSpread(const RowsArgs &a)
+    {
+        const int lane = threadIdx.x & 63;
+        item(a, lane);
+        unsigned t = lane < a.n ? T + RW_PAD : 0;
+        for (int b = 64; b < a.n; b += 64) {
+            int s;
+            if (b + lane < a.n) t += rows_tiles<TP>(a, rows_item(a, b + lane, &s)) + RW_PAD;
+        }
+        R = max(RW_RMIN, (wave_sum_u(t) + a.bal - 1) / a.bal);
+    }
+    __device__ __forceinline__ void item(const RowsArgs &a, int i)
+    {
+        slot = -1;
+        L = i < a.n ? rows_item(a, i, &slot) : 0;
+        T = rows_tiles<TP>(a, L);
+    }
+};
 
-// The piece of slot k: its item (-1: none) and the item's tiles [u0, u1);
-// whole: the item's only one.
-__device__ __forceinline__ int rows_piece(const RowsArgs &a, int k, int *u0, int *u1, bool *whole)
+struct RowsPiece {
+    int item, L, slot, u0, u1;   // item below 0: no piece
+    bool whole;                  // the item's only one
+};
+// The piece of work-group slot k, or item k whole where there are no ranges.
+template <int TP>
+__device__ __forceinline__ RowsPiece rows_piece(const RowsArgs &a, int k)
 {
+    RowsPiece p;
+    if (!a.bal) {
+        p.item = k;
+        p.L = rows_item(a, k, &p.slot);
+        p.u0 = 0;
+        p.u1 = rows_tiles<TP>(a, p.L);
+        p.whole = true;
+        return p;
+    }
     const int lane = threadIdx.x & 63;
-    const unsigned t0 = rows_tiles(a, lane);
-    const unsigned R = rows_range(a, t0);
+    RowsSpread<TP> x(a);
     unsigned base = 0;
+    p.item = -1;
     for (int b = 0; b < a.n; b += 64) {
-        const unsigned T = b == 0 ? t0 : rows_tiles(a, b + lane);
-        const unsigned v = b + lane < a.n ? T + RW_PAD : 0, inc = wave_scan_u(v);
+        if (b) x.item(a, b + lane);
+        const unsigned v = b + lane < a.n ? x.T + RW_PAD : 0, inc = wave_scan_u(v);
         const unsigned at = base + inc - v + RW_PAD;   // the item's first tile on the line
         const int w = k - (b + lane);
-        const uint64_t m = __ballot(T > 0 && w >= (int)(at / R) && w <= (int)((at + T - 1) / R));
+        const uint64_t m = __ballot(x.T > 0 && w >= (int)(at / x.R) && w <= (int)((at + x.T - 1) / x.R));
         if (m) {
             const int j = __builtin_ctzll(m), i = b + j;
-            const int n = __builtin_amdgcn_readlane(T, j);
-            const int r0 = (int)((unsigned)(k - i) * R - (unsigned)__builtin_amdgcn_readlane(at, j));
-            *u0 = max(r0, 0);
-            *u1 = min(r0 + (int)R, n);
-            *whole = r0 <= 0 && r0 + (int)R >= n;
-            return i;
+            const int n = __builtin_amdgcn_readlane(x.T, j);
+            const int r0 = (int)((unsigned)(k - i) * x.R - (unsigned)__builtin_amdgcn_readlane(at, j));
+            p.item = i;
+            p.L = __builtin_amdgcn_readlane(x.L, j);
+            p.slot = __builtin_amdgcn_readlane(x.slot, j);
+            p.u0 = max(r0, 0);
+            p.u1 = min(r0 + (int)x.R, n);
+            p.whole = r0 <= 0 && r0 + (int)x.R >= n;
+            break;
         }
         base += __builtin_amdgcn_readlane(inc, 63);
     }
-    return -1;
+    return p;
 }
 
 // The slots of item i's pieces: the first, and how many.
+template <int TP>
 __device__ __forceinline__ int rows_pieces(const RowsArgs &a, int i, int *first)
 {
+    int slot;
+    if (!a.bal) {
+        *first = i;
+        return rows_item(a, i, &slot) > 0 ? 1 : 0;
+    }
     const int lane = threadIdx.x & 63;
-    const unsigned t0 = rows_tiles(a, lane), R = rows_range(a, t0);
-    unsigned pre = 0;
-    for (int b = 0; b < i; b += 64) pre += b + lane < i ? (b == 0 ? t0 : rows_tiles(a, b + lane)) + RW_PAD : 0;
-    const unsigned at = wave_sum_u(pre) + RW_PAD, T = rows_tiles(a, i);
-    *first = (int)(at / R) + i;
-    return T ? (int)((at + T - 1) / R - at / R) + 1 : 0;
+    const unsigned T = rows_tiles<TP>(a, rows_item(a, i, &slot));
+    const RowsSpread<TP> x(a);
+    unsigned pre = lane < min(i, 64) ? x.T + RW_PAD : 0;
+    for (int b = 64; b < i; b += 64)
+        if (b + lane < i) pre += rows_tiles<TP>(a, rows_item(a, b + lane, &slot)) + RW_PAD;
+    const unsigned at = wave_sum_u(pre) + RW_PAD;
+    *first = (int)(at / x.R) + i;
+    return T ? (int)((at + T - 1) / x.R - at / x.R) + 1 : 0;
 }
 
 // ---- the walk ------------------------------------------------------------------
@@ -195,48 +234,60 @@ struct RowsWave {
     f32x4 o[RT][VD];         // o[rt][e][i]: dimension VD (4g + i) + e of the row
     float m[RT], mk[RT], l[RT];   // l: this lane's positions only
 
-    // row r's query at q(r)
+    // Row r's query at q(r): loaded first, made an operand once the first cached
+    // rows are on their way.
+    static constexpr int XR = F16 ? KS * 8 : VD * 4;
+    float x[RT][XR];
     template <typename Q>
-    __device__ __forceinline__ void start(Q q)
+    __device__ __forceinline__ void load(Q q)
     {
-#pragma clang fp contract(off)
         const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-        const float sc = 1.44269504088896341f / sqrtf((float)DH);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             const float *p = q(16 * rt + col);
+#pragma unroll
+            for (int i = 0; i < XR / 4; i++) {
+                const f32x4 y = F16 ? ldg((const f32x4 *)(p + (32 * (i / 2) + 8 * g) % DH + 4 * (i & 1)))
+                                    : ldg((const f32x4 *)(p + 16 * i + 4 * g));
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[rt][4 * i + e] = y[e];
+            }
+        }
+    }
+    __device__ __forceinline__ void convert()
+    {
+#pragma clang fp contract(off)
+        const int g = (threadIdx.x & 63) >> 4;
+        const float sc = 1.44269504088896341f / sqrtf((float)DH);
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
             c2[rt] = sc;
             if constexpr (F16) {
-                float x[KS][8], top = 0.0f;
+                float top = 0.0f;
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const float4 a = ldg((const float4 *)(p + (32 * s + 8 * g) % DH));
-                    const float4 b = ldg((const float4 *)(p + (32 * s + 8 * g) % DH + 4));
-                    const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        x[s][e] = DH < 32 && g >= 2 ? 0.0f : y[e];   // (d_head 16: half a k-step)
-                        top = fmaxf(top, fabsf(x[s][e]));
-                    }
+                for (int i = 0; i < XR; i++) {
+                    if (DH < 32 && g >= 2) x[rt][i] = 0.0f;   // (d_head 16: half a k-step)
+                    top = fmaxf(top, fabsf(x[rt][i]));
                 }
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
-                // the largest into [1, 2) (below 2^-100 less, so that c2 stays
-                // above 0); a row of zeros, infinities or NaN as it is
-                const int ex = top > 0.0f && top < INFINITY ? max(ilogbf(top), -100) : 0;
+                // the largest into [2^9, 2^10), so that the low parts are normal
+                // numbers too (below 2^-100 less, so that c2 stays above 0); a row
+                // of zeros, infinities or NaN as it is
+                const int ex = top > 0.0f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top) - 1, -100) - 9 : 0;
                 c2[rt] = ldexpf(sc, ex);
 #pragma unroll
                 for (int s = 0; s < KS; s++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
-                        const float y = ldexpf(x[s][e], -ex);
+                        const float y = __builtin_amdgcn_ldexpf(x[rt][8 * s + e], -ex);
                         const _Float16 hi = (_Float16)y;
                         qh[rt][s][e] = hi;
-                        ql[rt][s][e] = (_Float16)((y - (float)hi) * 2048.0f);
+                        ql[rt][s][e] = (_Float16)(y - (float)hi);
                     }
             } else {
 #pragma unroll
-                for (int i = 0; i < VD; i++) qf[rt][i] = ldg((const f32x4 *)(p + 16 * i + 4 * g));
+                for (int i = 0; i < VD; i++) qf[rt][i] = f32x4{x[rt][4 * i], x[rt][4 * i + 1], x[rt][4 * i + 2], x[rt][4 * i + 3]};
             }
             m[rt] = -INFINITY;
             mk[rt] = RW_SCALE;
@@ -253,30 +304,30 @@ struct RowsSeen {
     const int *pos;
 };
 
-// Tiles u, u + step, .. below u1 of `line` into the wave's rows, K and V rows
-// of the kv head at kb and vb.  MASKED: rows see different positions (seen).
+// Tiles u, u + step, .. below u1 of `line` into the wave's rows (loaded, not yet
+// converted), K and V rows of the kv head at kb and vb.  MASKED: rows see
+// different positions (seen).
 template <int DH, typename KT, int RT, bool MASKED>
-__device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb, const KT *vb, const RowsLine &line, int u,
-                                          int u1, int step, const RowsSeen *seen)
+__device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb, const KT *vb,
+                                          const RowsLine<rw_tp<KT>()> &line, int u, int u1, int step, const RowsSeen *seen)
 {
 #pragma clang fp contract(off)
     typedef RowsWave<DH, KT, RT> W;
     constexpr bool F16 = W::F16;
-    constexpr int VD = W::VD, KS = W::KS, ES = sizeof(KT);
+    constexpr int VD = W::VD, KS = W::KS, ES = sizeof(KT), TP = rw_tp<KT>(), C = TP / 16, VR = TP / 4;
     constexpr int VB = VD * ES;                        // bytes of a lane's piece of a V row
     constexpr int VW = VB < 4 ? 1 : VB / 4;            // dwords of it
     const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-    if (u >= u1) return;
     const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
-    f16x8 kh[F16 ? 2 : 1][F16 ? KS : 1];
-    f32x4 kf[F16 ? 1 : 2][F16 ? 1 : VD];
-    uint32_t vr[8][VW];                                // rows 4g + r (r < 4), 16 + 4g + r - 4
+    f16x8 kh[F16 ? C : 1][F16 ? KS : 1];
+    f32x4 kf[F16 ? 1 : VD];
+    uint32_t vr[VR][VW];                               // V rows 16 (r / 4) + 4g + r % 4
     auto load_k = [&](int t) {
         int p0, cnt;
         line.tile(t, &p0, &cnt);
         const char *base = (const char *)uniform_ptr(kb + (size_t)p0 * DH);
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
+        for (int c = 0; c < C; c++) {
             const unsigned at = (unsigned)min(16 * c + col, cnt - 1) * (DH * ES);
             if constexpr (F16) {
 #pragma unroll
@@ -286,7 +337,7 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < VD; i++) kf[c][i] = ldg((const f32x4 *)(base + (at + 64 * i + 16 * g)));
+                for (int i = 0; i < VD; i++) kf[i] = ldg((const f32x4 *)(base + (at + 64 * i + 16 * g)));
             }
         }
     };
@@ -295,8 +346,8 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
         line.tile(t, &p0, &cnt);
         const char *base = (const char *)uniform_ptr(vb + (size_t)p0 * DH);
 #pragma unroll
-        for (int r = 0; r < 8; r++) {
-            const int row = (r < 4 ? 0 : 12) + 4 * g + r;
+        for (int r = 0; r < VR; r++) {
+            const int row = 16 * (r / 4) + 4 * g + r % 4;
             const char *src = base + ((unsigned)min(row, cnt - 1) * (DH * ES) + VB * col);
             if constexpr (VB == 2) vr[r][0] = *gptr((const uint16_t *)src);
             else if constexpr (VB == 4) vr[r][0] = ldg((const uint32_t *)src);
@@ -314,48 +365,46 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
             }
         }
     };
-    load_k(u);
-    load_v(u);
+    if (u < u1) {
+        load_k(u);
+        load_v(u);
+    }
+    w.convert();
     for (; u < u1; u += step) {
         int p0, cnt;
         line.tile(u, &p0, &cnt);
         // ---- scores: sc[rt][c][i] = position p0 + 16c + 4g + i of row 16 rt + col
-        float sc[RT][2][4];
+        f32x4 sc[RT][C];
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
+        for (int c = 0; c < C; c++) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                f32x4 s1 = zero4;
+                sc[rt][c] = zero4;
                 if constexpr (F16) {
-                    f32x4 s2 = zero4;
 #pragma unroll
                     for (int s = 0; s < KS; s++) {
-                        s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.qh[rt][s], s1, 0, 0, 0);
-                        s2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.ql[rt][s], s2, 0, 0, 0);
+                        sc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.ql[rt][s], sc[rt][c], 0, 0, 0);
+                        sc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[c][s], w.qh[rt][s], sc[rt][c], 0, 0, 0);
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sc[rt][c][i] = fmaf(s2[i], 1.0f / 2048.0f, s1[i]);
                 } else {
 #pragma unroll
                     for (int d = 0; d < VD; d++)
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c][d][e], w.qf[rt][d][e], s1, 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) sc[rt][c][i] = s1[i];
+                            sc[rt][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[d][e], w.qf[rt][d][e], sc[rt][c], 0, 0, 0);
                 }
             }
         }
         if (u + step < u1) load_k(u + step);
         // ---- masks (uniform branches): the run's end; rows that see less
-        bool edge = cnt < RW_TP;
+        bool edge = cnt < TP;
         if constexpr (MASKED)
             edge |= p0 + cnt - 1 > seen->first || (p0 + cnt - 1 >= seen->sinks && p0 <= seen->last - seen->window);
         if (edge) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int c = 0; c < 2; c++)
+                for (int c = 0; c < C; c++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int at = 16 * c + 4 * g + i, p = p0 + at;
@@ -366,27 +415,32 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
                     }
         }
         // V rows past the run: 0, not a copy of its last (0 weight times infinity)
-        if (cnt < RW_TP) {
+        if (cnt < TP) {
 #pragma unroll
-            for (int r = 0; r < 8; r++)
-                if ((r < 4 ? 0 : 12) + 4 * g + r >= cnt) {
+            for (int r = 0; r < VR; r++)
+                if (16 * (r / 4) + 4 * g + r % 4 >= cnt) {
 #pragma unroll
                     for (int e = 0; e < VW; e++) vr[r][e] = 0;
                 }
         }
         // ---- online softmax
-        f16x8 ph[F16 ? RT : 1], pl[F16 ? RT : 1];
+        float mx[RT];
+        bool up = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            float mx = sc[rt][0][0];
+            mx[rt] = sc[rt][0][0];
 #pragma unroll
-            for (int c = 0; c < 2; c++)
+            for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[rt][c][i]);
-            if (__ballot((mx - w.m[rt]) * w.c2[rt] > RW_LAZY)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mn = fmaxf(w.m[rt], mx);
+                for (int i = 0; i < 4; i++) mx[rt] = fmaxf(mx[rt], sc[rt][c][i]);
+            up |= (mx[rt] - w.m[rt]) * w.c2[rt] > RW_LAZY;
+        }
+        if (__ballot(up)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 16, 64));
+                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 32, 64));
+                const float mn = fmaxf(w.m[rt], mx[rt]);
                 const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn * w.c2[rt];
                 const float al = w.m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - w.mk[rt]);
                 w.m[rt] = mn;
@@ -395,9 +449,13 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
 #pragma unroll
                 for (int e = 0; e < VD; e++) w.o[rt][e] *= al;
             }
+        }
+        f16x8 ph[F16 ? RT : 1], pl[F16 ? RT : 1];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
             float ls = 0.0f;
 #pragma unroll
-            for (int c = 0; c < 2; c++)
+            for (int c = 0; c < C; c++)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                     const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], w.c2[rt], w.mk[rt]));
@@ -428,19 +486,15 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
                     x[j] = __builtin_amdgcn_perm(vr[2 * j + 1][e / 2], vr[2 * j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
                 const f16x8 va = __builtin_bit_cast(f16x8, x);
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++) {
-                    w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[rt], w.o[rt][e], 0, 0, 0);
-                    w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[rt], w.o[rt][e], 0, 0, 0);
-                }
+                for (int rt = 0; rt < RT; rt++) w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[rt], w.o[rt][e], 0, 0, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[rt], w.o[rt][e], 0, 0, 0);
             } else {
 #pragma unroll
-                for (int c = 0; c < 2; c++)
+                for (int j = 0; j < 4; j++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++)
-                            w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[4 * c + j][e]), sc[rt][c][j],
-                                                                              w.o[rt][e], 0, 0, 0);
+                    for (int rt = 0; rt < RT; rt++)
+                        w.o[rt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][e]), sc[rt][0][j], w.o[rt][e], 0, 0, 0);
             }
         }
         if (u + step < u1) load_v(u + step);
@@ -448,22 +502,24 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
 }
 
 // The waves of a work-group meet: put(r, m, l, d, x) gets, for every row r of
-// the work-group's 16 RT, the rows' sums over the waves: weight sum l 2^m and
+// the work-group's 16 RT, its sums over the waves: weight sum l 2^m and
 // the unnormalised output's dimensions d .. d+N-1 (x), from one thread each.
-template <int DH>
+template <int DH, int NW>
 struct RowsMeet {
-    static constexpr int DC = DH < 128 ? DH : 128;   // dimensions per round
-    __attribute__((aligned(16))) float o[RW_NW][16][DC + 4];
-    float m[RW_NW][16], l[RW_NW][16];
+    static constexpr int DC = DH < 512 / NW ? DH : 512 / NW;   // dimensions per round (34 KiB)
+    __attribute__((aligned(16))) float o[NW][16][DC + 4];
+    float m[NW][16], l[NW][16];
 };
-template <int DH, typename KT, int RT, typename P>
-__device__ __forceinline__ void rows_finish(RowsWave<DH, KT, RT> &w, RowsMeet<DH> &meet, P put)
+template <int DH, typename KT, int RT, int NW, typename P>
+__device__ __forceinline__ void rows_finish(RowsWave<DH, KT, RT> &w, RowsMeet<DH, NW> &meet, P put)
 {
-    constexpr int VD = DH / 16, DC = RowsMeet<DH>::DC, N = DC / 16;   // dimensions per thread and round
+#pragma clang fp contract(off)
+    constexpr int VD = DH / 16, DC = RowsMeet<DH, NW>::DC, TPR = NW * 4;   // threads per row
+    constexpr int N = DC / TPR < 1 ? 1 : DC / TPR;                        // dimensions per thread and round
     auto &xo = meet.o;
     auto &xm = meet.m, &xl = meet.l;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, col = lane & 15, g = lane >> 4;
-    const int r = tid >> 4, a = tid & 15;
+    const int r = tid / TPR, a = tid % TPR;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         float l = w.l[rt];
@@ -486,17 +542,18 @@ __device__ __forceinline__ void rows_finish(RowsWave<DH, KT, RT> &w, RowsMeet<DH
             __syncthreads();
             float mx = xm[0][r];
 #pragma unroll
-            for (int k = 1; k < RW_NW; k++) mx = fmaxf(mx, xm[k][r]);
+            for (int k = 1; k < NW; k++) mx = fmaxf(mx, xm[k][r]);
             const float ref = mx == -INFINITY ? 0.0f : mx;
             float lt = 0.0f, x[N] = {};
+            const bool on = N * a < DC;   // (d_head 16 over eight waves: half of the threads)
 #pragma unroll
-            for (int k = 0; k < RW_NW; k++) {
+            for (int k = 0; k < NW; k++) {
                 const float f = __builtin_amdgcn_exp2f(xm[k][r] - ref);
                 lt += xl[k][r] * f;
 #pragma unroll
-                for (int e = 0; e < N; e++) x[e] += xo[k][r][N * a + e] * f;
+                for (int e = 0; e < N; e++) x[e] += on ? xo[k][r][N * a + e] * f : 0.0f;
             }
-            put(16 * rt + r, mx, lt, c * DC + N * a, x);
+            if (on) put(16 * rt + r, mx, lt, c * DC + N * a, x);
         }
     }
 }
@@ -616,9 +673,10 @@ constexpr int RW_WGS = 512;   // work-groups of a call to aim for: two per CU
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 // Balanced ranges for n items of up to `span` tiles on `heads` work-groups
-// each: 0 (an item whole) where an item has at most two rounds of tiles for its
-// waves or the items alone fill the chip.
-int rows_plan_bal(int n, long heads, long span);
+// each, 0 (an item whole) where the items alone fill the chip or an item has at
+// most `whole` tiles.  (Tiles of 32 positions: a plan serves both cache types.)
+constexpr int RW_PLAN_TP = 32;
+int rows_plan_bal(int n, long heads, long span, long whole);
 
 // What a call of these shapes splits into, and the number of its partial
 // results.

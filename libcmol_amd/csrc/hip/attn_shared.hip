@@ -7,6 +7,8 @@
 // takes the parts and the pieces of a row.
 #include "attn_rows.h"
 
+constexpr int SH_NW = 4;   // waves per work-group
+
 // work-groups of the prefix: (kv head, part) fastest, padded to the eight XCDs,
 // so the row blocks that read the same positions run on one XCD and its L2
 __host__ __device__ inline unsigned shared_lanes(const RowsArgs &a) { return (unsigned)(a.n_kv * a.parts + 7) / 8 * 8; }
@@ -17,7 +19,7 @@ __host__ __device__ inline unsigned shared_prefix_wgs(const RowsArgs &a, int rt)
 }
 
 template <int DH, typename KT, int RT>
-__device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH> &meet, unsigned wg)
+__device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH, SH_NW> &meet, unsigned wg)
 {
 #pragma clang fp contract(off)
     const int G = a.n_heads / a.n_kv, rows = a.n * G;
@@ -25,18 +27,18 @@ __device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH> &m
     const int kvh = lane / a.parts, part = lane % a.parts, r0 = wg / lanes * 16 * RT;
     if (kvh >= a.n_kv) return;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    RowsLine line;
+    RowsLine<rw_tp<KT>()> line;
     line.s = line.lo = line.ns = 0;
     line.hi = a.prefix;
     const int T = line.tiles(), R = (T + a.parts - 1) / a.parts;
     const int u0 = min(part * R, T), u1 = min(u0 + R, T);
     RowsWave<DH, KT, RT> w;
-    w.start([&](int r) {
+    w.load([&](int r) {
         r = min(r0 + r, rows - 1);
         return a.q + ((size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G) * DH;
     });
     const size_t base = (size_t)kvh * a.prefix_ctx * DH;
-    rows_walk<DH, KT, RT, false>(w, (const KT *)a.pk + base, (const KT *)a.pv + base, line, u0 + wid, u1, RW_NW, nullptr);
+    rows_walk<DH, KT, RT, false>(w, (const KT *)a.pk + base, (const KT *)a.pv + base, line, u0 + wid, u1, SH_NW, nullptr);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         if (r0 + r >= rows) return;
@@ -50,28 +52,21 @@ __device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH> &m
 }
 
 template <int DH, typename KT>
-__device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH> &meet, unsigned wg)
+__device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH, SH_NW> &meet, unsigned wg)
 {
 #pragma clang fp contract(off)
     const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
     const int slot = wg / (a.n_kv * blocks), hb = wg % (a.n_kv * blocks), kvh = hb / blocks, r0 = hb % blocks * 16;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int i = slot, u0 = 0, u1 = 0;
-    bool whole;
-    if (a.bal) {
-        i = rows_piece(a, slot, &u0, &u1, &whole);
-        if (i < 0) return;
-    }
-    size_t base;
-    const int L = rows_item(a, i, &base);
-    if (L <= 0) return;
-    const RowsLine line = rows_line(L - 1, L - 1, a.window, a.sinks);
-    if (!a.bal) u1 = line.tiles();
-    const size_t row0 = (size_t)i * a.n_heads + (size_t)kvh * G;
+    constexpr int TP = rw_tp<KT>();
+    const RowsPiece p = rows_piece<TP>(a, slot);
+    if (p.item < 0 || p.L <= 0) return;
+    const RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
+    const size_t row0 = (size_t)p.item * a.n_heads + (size_t)kvh * G;
     RowsWave<DH, KT, 1> w;
-    w.start([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
-    base += (size_t)kvh * a.max_ctx * DH;
-    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, u0 + wid, u1, RW_NW, nullptr);
+    w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
+    const size_t base = (size_t)p.slot * a.slot_stride + (size_t)kvh * a.max_ctx * DH;
+    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, p.u0 + wid, p.u1, SH_NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         r += r0;
@@ -85,26 +80,22 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH> &meet
 }
 
 template <int DH, typename KT, int RT>
-__global__ __launch_bounds__(256) void k_shared(RowsArgs a)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_shared(RowsArgs a)
 {
-    __shared__ RowsMeet<DH> meet;
+    __shared__ RowsMeet<DH, SH_NW> meet;
     const unsigned pre = shared_prefix_wgs(a, RT);
     if (blockIdx.x < pre) shared_prefix<DH, KT, RT>(a, meet, blockIdx.x);
     else shared_own<DH, KT>(a, meet, blockIdx.x - pre);
 }
 
-template <int DH>
+template <int DH, int TP>
 __global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
 {
     constexpr int LPR = DH / 4;
     const int G = a.n_heads / a.n_kv, h = blockIdx.x, kvh = h / G, i = blockIdx.y, tid = threadIdx.x;
     const int pre = a.prefix ? a.parts : 0;
-    int first = i, np;
-    if (a.bal) np = rows_pieces(a, i, &first);
-    else {
-        size_t base;
-        np = rows_item(a, i, &base) > 0 ? 1 : 0;
-    }
+    int first;
+    const int np = rows_pieces<TP>(a, i, &first);
     const size_t x0 = ((size_t)kvh * a.n * G + (size_t)i * G + h % G) * a.parts;
     const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
     const f32x4 o = rows_sum<DH, 256 / LPR>(
@@ -129,7 +120,7 @@ static int shared_rt(int n, int G, int d_head, int kv_f16)
 static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt)
 {
     const long blocks = (long)n_kv * ceil_div((long)n * (n_heads / n_kv), 16 * rt);
-    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_TP), RW_NW)));
+    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_PLAN_TP), SH_NW)));
 }
 
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
@@ -140,7 +131,7 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
     for (int f16 = 0; f16 < 2; f16++)
         p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16)));
     p.cross = prefix ? (size_t)n * n_heads * p.parts : 0;
-    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_TP));
+    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP), 8);
     p.pieces = (size_t)n_kv * (p.bal + n) * G;
     return p;
 }
@@ -163,7 +154,9 @@ int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
     RW_BY_D_HEAD(a.d_head, SHA)
 #undef SHA
 #undef LAUNCH
-#define MERGE(DH) hipLaunchKernelGGL(k_shared_merge<DH>, dim3(a.n_heads, a.n), block, 0, s, a);
+#define MERGE(DH)                                                                                     \
+    if (a.kv_f16) hipLaunchKernelGGL((k_shared_merge<DH, 32>), dim3(a.n_heads, a.n), block, 0, s, a); \
+    else hipLaunchKernelGGL((k_shared_merge<DH, 16>), dim3(a.n_heads, a.n), block, 0, s, a);
     RW_BY_D_HEAD(a.d_head, MERGE)
 #undef MERGE
     return hipGetLastError() == hipSuccess ? 0 : -4;

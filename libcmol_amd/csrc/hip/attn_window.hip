@@ -4,38 +4,32 @@
 
 // ---- single tokens ---------------------------------------------------------------
 
-// Work-group (16 query heads of a kv head, slot): the piece of that slot, or
-// item `slot` whole where there are no balanced ranges.
-template <int DH, typename KT>
-__global__ __launch_bounds__(256) void k_window(RowsArgs a)
+// Work-group of NW waves (16 query heads of a kv head, slot): the piece of that
+// slot, or item `slot` whole where there are no balanced ranges.
+template <int DH, typename KT, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window(RowsArgs a)
 {
 #pragma clang fp contract(off)
-    __shared__ RowsMeet<DH> meet;
+    constexpr int TP = rw_tp<KT>();
+    __shared__ RowsMeet<DH, NW> meet;
     const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
     const int kvh = blockIdx.x / blocks, r0 = (blockIdx.x % blocks) * 16, slot = blockIdx.y;
     const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int i = slot, u0 = 0, u1 = 0;
-    bool whole = true;
-    if (a.bal) {
-        i = rows_piece(a, slot, &u0, &u1, &whole);
-        if (i < 0) return;
-    }
-    size_t base;
-    const int L = rows_item(a, i, &base);
-    const RowsLine line = rows_line(L - 1, L - 1, a.window, a.sinks);
-    if (!a.bal) u1 = L > 0 ? line.tiles() : 0;
-    const size_t row0 = (size_t)i * a.n_heads + (size_t)kvh * G;
+    const RowsPiece p = rows_piece<TP>(a, slot);
+    if (p.item < 0) return;
+    const RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
+    const size_t row0 = (size_t)p.item * a.n_heads + (size_t)kvh * G;
     RowsWave<DH, KT, 1> w;
-    w.start([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
-    base += (size_t)kvh * a.max_ctx * DH;
-    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, u0 + wid, u1, RW_NW, nullptr);
+    w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
+    const size_t base = (p.L > 0 ? (size_t)p.slot * a.slot_stride : 0) + (size_t)kvh * a.max_ctx * DH;
+    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, p.u0 + wid, p.u1, NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
-        if (whole) {
-            const float f = L > 0 ? 1.0f / l : 0.0f;
-            for (auto &y : x) y = L > 0 ? y * f : 0.0f;
+        if (p.whole) {
+            const float f = p.L > 0 ? 1.0f / l : 0.0f;
+            for (auto &y : x) y = p.L > 0 ? y * f : 0.0f;
             rows_store(a.out + (row0 + r) * DH + d, x);
         } else {
             rows_store(a.po + (part + r) * DH + d, x);
@@ -48,13 +42,13 @@ __global__ __launch_bounds__(256) void k_window(RowsArgs a)
 }
 
 // One work-group per (query head, item): the item's pieces.
-template <int DH>
+template <int DH, int TP>
 __global__ __launch_bounds__(256) void k_window_merge(RowsArgs a)
 {
     constexpr int LPR = DH / 4;
     const int G = a.n_heads / a.n_kv, h = blockIdx.x, kvh = h / G, i = blockIdx.y, tid = threadIdx.x;
     int first;
-    const int np = rows_pieces(a, i, &first);
+    const int np = rows_pieces<TP>(a, i, &first);
     if (np == 1) return;   // finished by its only piece
     const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
     const f32x4 o = rows_sum<DH, 256 / LPR>(np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
@@ -75,7 +69,8 @@ template <int DH, typename KT, int RT>
 __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
 {
 #pragma clang fp contract(off)
-    __shared__ RowsMeet<DH> meet;
+    constexpr int TP = rw_tp<KT>(), NW = 4;
+    __shared__ RowsMeet<DH, NW> meet;
     __shared__ int odd;
     const int G = a.n_heads / a.n_kv, rows = a.n * G;
     const int kvh = blockIdx.x % a.n_kv, r0 = blockIdx.x / a.n_kv * 16 * RT, part = blockIdx.y;
@@ -86,7 +81,7 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     seen.last = a.pos0 + (r0 + nr - 1) / G;
     seen.window = a.window;
     seen.sinks = a.sinks;
-    const RowsLine line = rows_line(seen.first, seen.last, a.window, a.sinks);
+    const RowsLine<TP> line = rows_line<TP>(seen.first, seen.last, a.window, a.sinks);
     const int T = line.tiles(), R = (T + a.parts - 1) / a.parts;
     const int u0 = min(part * R, T), u1 = min(u0 + R, T);
     int pos[RT];
@@ -100,10 +95,10 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     const size_t base = (size_t)kvh * a.max_ctx * DH;
     const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
     RowsWave<DH, KT, RT> w;
-    w.start([&](int r) { return a.q + row_at(r) * DH; });
+    w.load([&](int r) { return a.q + row_at(r) * DH; });
     if (tid == 0) odd = 0;
     __syncthreads();
-    rows_walk<DH, KT, RT, true>(w, k, v, line, u0 + wid, u1, RW_NW, &seen);
+    rows_walk<DH, KT, RT, true>(w, k, v, line, u0 + wid, u1, NW, &seen);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
     bool bad = false;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
@@ -132,7 +127,7 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     if (!odd) return;
     constexpr int DL = RowState<DH>::DL;
     const bool on = lane * DL < DH;
-    for (int r = wid; r < nr; r += RW_NW) {
+    for (int r = wid; r < nr; r += NW) {
         const size_t qa = row_at(r) * DH + (on ? lane * DL : 0);
         const int p = a.pos0 + (r0 + r) / G;
         RowState<DH> t;
@@ -170,21 +165,25 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
 static long span_tiles(int max_ctx, int window, int sinks)
 {
     const long w = std::min(window, max_ctx), s = std::min(sinks, max_ctx);
-    return std::min((long)ceil_div(w, RW_TP) + ceil_div(s, RW_TP), (long)ceil_div(max_ctx, RW_TP) + 2);
+    return std::min((long)ceil_div(w, RW_PLAN_TP) + ceil_div(s, RW_PLAN_TP), (long)ceil_div(max_ctx, RW_PLAN_TP) + 2);
 }
 
-int rows_plan_bal(int n, long heads, long span)
+int rows_plan_bal(int n, long heads, long span, long whole)
 {
-    if (span <= 2 * RW_NW || n * heads >= RW_WGS || n * (span + RW_PAD) > INT32_MAX) return 0;
+    if (span <= whole || n * heads >= RW_WGS || n * (span + RW_PAD) > INT32_MAX / 4) return 0;
     const long want = std::max(1L, RW_WGS / heads - n);
     return (int)std::min(want, n * (long)ceil_div(span + RW_PAD, RW_RMIN));
 }
+
+// An item of up to this many tiles is one work-group's, of eight waves: the
+// waves' rounds cost less than a merge launch.
+constexpr int WIN_WHOLE = 32;
 
 RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks)
 {
     RowsPlan p;
     const int G = n_heads / n_kv;
-    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks));
+    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks), WIN_WHOLE);
     if (p.bal) p.pieces = (size_t)n_kv * (p.bal + n) * G;
     return p;
 }
@@ -199,8 +198,8 @@ static int prompt_parts(int n, int n_heads, int n_kv, int max_ctx, int window, i
 {
     const int G = n_heads / n_kv;
     const long blocks = (long)n_kv * ceil_div((long)n * G, 16 * rt);
-    const long span = std::min(span_tiles(max_ctx, window, sinks) + ceil_div(16 * rt, G * RW_TP) + 1, (long)ceil_div(max_ctx, RW_TP) + 2);
-    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(span, 2 * RW_NW)));
+    const long span = std::min(span_tiles(max_ctx, window, sinks) + ceil_div(16 * rt, G * RW_PLAN_TP) + 1, (long)ceil_div(max_ctx, RW_PLAN_TP) + 2);
+    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(span, 8)));
 }
 
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
@@ -218,14 +217,23 @@ RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx,
 
 int launch_attn_window(const RowsArgs &a, hipStream_t s)
 {
-    const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), a.bal + a.n), block(256);
-#define WIN(DH)                                                                          \
-    if (a.kv_f16) hipLaunchKernelGGL((k_window<DH, _Float16>), grid, block, 0, s, a);    \
-    else hipLaunchKernelGGL((k_window<DH, float>), grid, block, 0, s, a);
+    const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), a.bal + a.n);
+    // eight waves for items that have more than one round of tiles for four
+    // (d_head 256: four, for their registers)
+    const bool wide = !a.bal && a.d_head < 256 && span_tiles(a.max_ctx, a.window, a.sinks) > 4;
+#define LAUNCH(DH, KT, NW) hipLaunchKernelGGL((k_window<DH, KT, NW>), grid, dim3(NW * 64), 0, s, a)
+#define WIN(DH)                                                               \
+    if constexpr (DH < 256) {                                                 \
+        if (wide) { if (a.kv_f16) LAUNCH(DH, _Float16, 8); else LAUNCH(DH, float, 8); }   \
+    }                                                                         \
+    if (!wide) { if (a.kv_f16) LAUNCH(DH, _Float16, 4); else LAUNCH(DH, float, 4); }
     RW_BY_D_HEAD(a.d_head, WIN)
 #undef WIN
+#undef LAUNCH
     if (a.bal) {
-#define MERGE(DH) hipLaunchKernelGGL(k_window_merge<DH>, dim3(a.n_heads, a.n), block, 0, s, a);
+#define MERGE(DH)                                                                                              \
+    if (a.kv_f16) hipLaunchKernelGGL((k_window_merge<DH, 32>), dim3(a.n_heads, a.n), dim3(256), 0, s, a);      \
+    else hipLaunchKernelGGL((k_window_merge<DH, 16>), dim3(a.n_heads, a.n), dim3(256), 0, s, a);
         RW_BY_D_HEAD(a.d_head, MERGE)
 #undef MERGE
     }
