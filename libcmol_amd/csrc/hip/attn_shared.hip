@@ -109,18 +109,24 @@ __global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
     if (tid < LPR) *(f32x4 *)(a.out + ((size_t)i * a.n_heads + h) * DH + 4 * tid) = o;
 }
 
-// Row tiles of a prefix work-group: as many as the registers hold, no more than
-// there are rows.
+// Row tiles of a prefix work-group: two over fp16 where there are rows for them
+// and registers (a position read once for 32 rows), one over fp32, whose
+// products take sixteen times as long and spread better in small pieces (48
+// sessions of 4 heads behind 2000 positions: 22.1 against 23.2 us).
 static int shared_rt(int n, int G, int d_head, int kv_f16)
 {
-    const long rows = (long)n * G;
-    return std::min(rows <= 16 ? 1 : rows <= 32 ? 2 : 4, d_head == 256 ? 1 : kv_f16 && d_head < 128 ? 4 : 2);
+    return (long)n * G <= 16 || d_head == 256 || !kv_f16 ? 1 : 2;
 }
+
+// Work-groups of the prefix to aim for: with those of the own positions one
+// round of two per CU (32 sessions of 4 heads behind 8192 positions, fp16: 24.6
+// us at 96, 20.5 at 160, 23.5 at 224, 26.4 at 512).
+constexpr int SH_PREFIX_WGS = 192;
 
 static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt)
 {
     const long blocks = (long)n_kv * ceil_div((long)n * (n_heads / n_kv), 16 * rt);
-    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_PLAN_TP), SH_NW)));
+    return (int)std::max(1L, std::min(SH_PREFIX_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_PLAN_TP), SH_NW)));
 }
 
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
@@ -144,16 +150,12 @@ int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
     const size_t wgs = shared_prefix_wgs(a, rt) + (size_t)a.n_kv * ceil_div(G, 16) * (a.bal + a.n);
     if (wgs > INT32_MAX) return -6;
     const dim3 grid((unsigned)wgs), block(256);
-#define LAUNCH(DH, KT, RT) hipLaunchKernelGGL((k_shared<DH, KT, RT>), grid, block, 0, s, a)
-#define SHA(DH)                                                                               \
-    if (rt == 1) { if (a.kv_f16) LAUNCH(DH, _Float16, 1); else LAUNCH(DH, float, 1); }        \
-    else if constexpr (DH < 256) {                                                            \
-        if (a.kv_f16) { if (rt == 2) LAUNCH(DH, _Float16, 2); else LAUNCH(DH, _Float16, 4); } \
-        else LAUNCH(DH, float, 2);                                                            \
-    }
+#define SHA(DH)                                                                                          \
+    if (!a.kv_f16) hipLaunchKernelGGL((k_shared<DH, float, 1>), grid, block, 0, s, a);                   \
+    else if (DH == 256 || rt == 1) hipLaunchKernelGGL((k_shared<DH, _Float16, 1>), grid, block, 0, s, a); \
+    else hipLaunchKernelGGL((k_shared<DH, _Float16, DH == 256 ? 1 : 2>), grid, block, 0, s, a);
     RW_BY_D_HEAD(a.d_head, SHA)
 #undef SHA
-#undef LAUNCH
 #define MERGE(DH)                                                                                     \
     if (a.kv_f16) hipLaunchKernelGGL((k_shared_merge<DH, 32>), dim3(a.n_heads, a.n), block, 0, s, a); \
     else hipLaunchKernelGGL((k_shared_merge<DH, 16>), dim3(a.n_heads, a.n), block, 0, s, a);

@@ -20,6 +20,6 @@ struct LogitsArgs {
     unsigned long long *part;       // [n][slabs] argmax keys (next wanted)
 };
 
-// Vocabulary slabs per row.
+// Most vocabulary slabs of a row.
 int logits_slabs(int vocab);
 int launch_logits(const LogitsArgs &a, hipStream_t s);

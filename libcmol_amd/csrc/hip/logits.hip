@@ -8,16 +8,17 @@
 // The repeat penalty is applied an occurrence at a time, each result rounded
 // to fp32, as cmol_apply_repeat_penalty does.
 //
-// One work-group per (slab of SLAB tokens, row): the slab's occurrences are
-// counted in LDS from the row's whole history (integer counts: the order of
-// the atomics does not matter), and of a token's bias entries the last is kept
-// (a maximum over their places).  The largest (value, lowest token) of a slab
-// goes to `part`; k_logits_pick takes the row's.
+// One work-group per (slab of the vocabulary, row).  The slab's logits and mask
+// words are requested first; meanwhile its occurrences are counted in LDS from
+// the row's whole history (integer counts: the order of the atomics does not
+// matter), and of a token's bias entries the last is kept (a maximum over their
+// places).  The largest (value, lowest token) of a slab goes to `part` and
+// k_logits_pick takes the row's.
+//
+// Bound: the logits read and written once, above the launches' few microseconds;
+// every work-group reads the row's history, so where the rows alone give each CU
+// one slabs are large (SLAB 8192 on 1024 threads), else small (2048 on 256).
 #include "logits.h"
-
-constexpr int SLAB = 2048;
-
-int logits_slabs(int vocab) { return (vocab + SLAB - 1) / SLAB; }
 
 __device__ inline unsigned long long key_max(unsigned long long k)
 {
@@ -30,71 +31,177 @@ __device__ inline unsigned long long key_max(unsigned long long k)
     return k;
 }
 
-__global__ __launch_bounds__(256) void k_logits(LogitsArgs a)
+// x / rep rounded, y = 1 / rep rounded, for 2^-60 <= x <= 2^100 and rep <= 2^30
+// (every step stays among the normal numbers): the quotient by y is within 1.5
+// ulp, one correction brings it within one, and with the remainder then exact a
+// second one rounds it as the division does (Markstein).
+__device__ inline float divide_step(float x, float rep, float y)
+{
+    float q = x * y;
+    q = fmaf(fmaf(-rep, q, x), y, q);
+    return fmaf(fmaf(-rep, q, x), y, q);
+}
+
+// The repeat penalty of c occurrences.  Eight steps at a time where there are
+// as many: a word that fills its history is a chain of hundreds of dependent
+// steps on one lane (32 rows, 211 occurrences at most: 11 us with a check a step).
+__device__ inline float repeat_penalty(float x, int c, float rep, float y)
 {
 #pragma clang fp contract(off)
-    __shared__ int cnt[SLAB], last[SLAB];
-    __shared__ unsigned long long best[4];
+    if (x > 0.0f) {
+        for (; c >= 8 && x >= 0x1p-28f && x <= 0x1p+100f && rep <= 16.0f; c -= 8)
+#pragma unroll
+            for (int i = 0; i < 8; i++) x = divide_step(x, rep, y);
+        for (; c > 0 && x >= 0x1p-60f && x <= 0x1p+100f && rep <= 0x1p+30f; c--) x = divide_step(x, rep, y);
+        for (; c > 0; c--) {
+            const float q = x / rep;
+            if (q == x) break;   // every further one leaves it
+            x = q;
+        }
+        return x;
+    }
+    for (; c >= 8; c -= 8) {
+        const float was = x;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x *= rep;
+        if (x == was) return x;
+    }
+    for (; c > 0; c--) x *= rep;
+    return x;
+}
+
+template <int SLAB, int NT>
+__global__ __launch_bounds__(NT) void k_logits(LogitsArgs a)
+{
+#pragma clang fp contract(off)
+    constexpr int Q = SLAB / NT / 4;   // fours of tokens per thread
+    __shared__ __attribute__((aligned(16))) int cnt[SLAB], last[SLAB];
+    __shared__ unsigned long long best[NT / 64];
     const int row = blockIdx.y, v0 = blockIdx.x * SLAB, nv = min(SLAB, a.vocab - v0), tid = threadIdx.x;
     const int hl = a.history ? min(max(a.history_len[row], 0), a.history_cap) : 0;
     const int bl = a.bias_ids ? min(max(a.bias_len[row], 0), a.bias_cap) : 0;
-    const int32_t *hist = a.history + (size_t)row * a.history_cap;
-    const int32_t *bids = a.bias_ids + (size_t)row * a.bias_cap;
-    const float *bias = a.bias + (size_t)row * a.bias_cap;
-    for (int i = tid; i < SLAB; i += 256) cnt[i] = last[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < hl; i += 256) {
-        const unsigned u = (unsigned)(hist[i] - v0);
-        if (hist[i] >= 0 && u < (unsigned)nv) atomicAdd(&cnt[u], 1);
-    }
-    for (int i = tid; i < bl; i += 256) {
-        const unsigned u = (unsigned)(bids[i] - v0);
-        if (bids[i] >= 0 && u < (unsigned)nv) atomicMax(&last[u], i + 1);
-    }
-    __syncthreads();
-    const float rep = a.repeat ? a.repeat[row] : 1.0f;
-    const float frq = a.frequency ? a.frequency[row] : 0.0f, prs = a.presence ? a.presence[row] : 0.0f;
     const int mr = !a.mask ? -1 : a.mask_row ? a.mask_row[row] : row;
     const bool masked = mr >= 0 && mr < a.mask_rows;
-    const uint32_t *mask = a.mask + (masked ? (size_t)mr * ((a.vocab + 31) / 32) : 0);
+    const float rep = a.repeat ? a.repeat[row] : 1.0f;
+    const float frq = a.frequency ? a.frequency[row] : 0.0f, prs = a.presence ? a.presence[row] : 0.0f;
+    const float *px = a.x + row * a.stride + v0;
+    float *po = a.out ? a.out + row * a.stride + v0 : nullptr;
+    const bool wide = (((uintptr_t)px | (uintptr_t)po) & 15) == 0;   // (uniform; v0 is a multiple of four)
+    const uint32_t *mask = a.mask + (masked ? (size_t)mr * ((a.vocab + 31) / 32) : 0) + v0 / 32;
+
+    // this thread's tokens 4 (tid + NT q) .. +3 of the slab (past nv: not used)
+    f32x4 x[Q];
+    uint32_t mw[Q];
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const int i = 4 * (tid + NT * q);
+        mw[q] = masked && i < nv ? mask[i >> 5] >> (i & 31) : ~0u;
+        if (wide && i + 4 <= nv) x[q] = *(const f32x4 *)(px + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[q][e] = i + e < nv ? px[i + e] : 0.0f;
+    }
+    if (hl | bl) {   // (uniform)
+        const u32x4 z = {};
+#pragma unroll
+        for (int q = 0; q < Q; q++) {
+            *(u32x4 *)&cnt[4 * (tid + NT * q)] = z;
+            if (bl) *(u32x4 *)&last[4 * (tid + NT * q)] = z;
+        }
+        __syncthreads();
+        const int32_t *hist = a.history + (size_t)row * a.history_cap;
+        auto count = [&](int id) {
+            const unsigned u = (unsigned)(id - v0);
+            if (id >= 0 && u < (unsigned)nv) atomicAdd(&cnt[u], 1);
+        };
+        int i = tid;
+        for (; i + 3 * NT < hl; i += 4 * NT) {   // four loads in one round trip
+            const int t0 = hist[i], t1 = hist[i + NT], t2 = hist[i + 2 * NT], t3 = hist[i + 3 * NT];
+            count(t0);
+            count(t1);
+            count(t2);
+            count(t3);
+        }
+        for (; i < hl; i += NT) count(hist[i]);
+        const int32_t *ids = a.bias_ids + (size_t)row * a.bias_cap;
+        for (int j = tid; j < bl; j += NT) {
+            const int id = ids[j];
+            const unsigned u = (unsigned)(id - v0);
+            if (id >= 0 && u < (unsigned)nv) atomicMax(&last[u], j + 1);
+        }
+        __syncthreads();
+    }
+    const float y = rep > 1.0f ? 1.0f / rep : 1.0f;
+    const float *bias = a.bias + (size_t)row * a.bias_cap;
     unsigned long long top = 0;
-    for (int i = tid; i < nv; i += 256) {
-        const int v = v0 + i;
-        float x = a.x[row * a.stride + v];
-        const int c = cnt[i];
-        if (rep > 1.0f) {
-            for (int j = 0; j < c; j++) {
-                const float y = x > 0.0f ? x / rep : x * rep;
-                if (y == x) break;   // 0 or an infinity: every further one leaves it
-                x = y;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+        const int i = 4 * (tid + NT * q);
+        if (hl) {
+            const u32x4 c4 = *(const u32x4 *)&cnt[i];
+            if (c4[0] | c4[1] | c4[2] | c4[3]) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int c = (int)c4[e];
+                    if (c && rep > 1.0f) x[q][e] = repeat_penalty(x[q][e], c, rep, y);
+                    if (c) x[q][e] -= frq * (float)c + prs;
+                }
             }
         }
-        if (c) x -= frq * (float)c + prs;
-        if (last[i]) x += bias[last[i] - 1];
-        if (masked && !((mask[v >> 5] >> (v & 31)) & 1)) x = -INFINITY;
-        if (a.out) a.out[row * a.stride + v] = x;
-        if (x > -INFINITY) top = max(top, argmax_key(x + 0.0f, (uint32_t)v));   // (never a NaN; -0 as 0)
+        if (bl) {
+            const u32x4 l4 = *(const u32x4 *)&last[i];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (l4[e]) x[q][e] += bias[l4[e] - 1];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (!((mw[q] >> e) & 1)) x[q][e] = -INFINITY;
+        if (po) {
+            if (wide && i + 4 <= nv) *(f32x4 *)(po + i) = x[q];
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (i + e < nv) po[i + e] = x[q][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {   // (never a NaN; -0 as 0)
+            const unsigned long long k = argmax_key(x[q][e] + 0.0f, (uint32_t)(v0 + i + e));
+            if (i + e < nv && x[q][e] > -INFINITY && k > top) top = k;
+        }
     }
     if (!a.next) return;
     top = key_max(top);
     if ((tid & 63) == 0) best[tid >> 6] = top;
     __syncthreads();
-    if (tid == 0) a.part[(size_t)row * gridDim.x + blockIdx.x] = max(max(best[0], best[1]), max(best[2], best[3]));
+    if (tid >= 64) return;
+    top = key_max(tid < NT / 64 ? best[tid] : 0);
+    if (tid == 0) a.part[(size_t)row * gridDim.x + blockIdx.x] = top;
 }
 
 __global__ __launch_bounds__(64) void k_logits_pick(LogitsArgs a, int slabs)
 {
     const int row = blockIdx.x;
     unsigned long long top = 0;
-    for (int i = threadIdx.x; i < slabs; i += 64) top = max(top, a.part[(size_t)row * slabs + i]);
+    for (int i = threadIdx.x; i < slabs; i += 64) {
+        const unsigned long long k = a.part[(size_t)row * slabs + i];
+        top = k > top ? k : top;
+    }
     top = key_max(top);
     if (threadIdx.x == 0) a.next[row] = top ? (int)argmax_index(top) : -1;
 }
 
+constexpr int SLAB_MIN = 2048, SLAB_MAX = 8192;
+
+int logits_slabs(int vocab) { return (vocab - 1) / SLAB_MIN + 1; }
+
 int launch_logits(const LogitsArgs &a, hipStream_t s)
 {
-    const int slabs = logits_slabs(a.vocab);
-    hipLaunchKernelGGL(k_logits, dim3(slabs, a.n), dim3(256), 0, s, a);
+    const int big = (a.vocab - 1) / SLAB_MAX + 1;
+    const bool large = (long)big * a.n >= 256;
+    const int slabs = large ? big : logits_slabs(a.vocab);
+    if (large) hipLaunchKernelGGL((k_logits<SLAB_MAX, 1024>), dim3(slabs, a.n), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((k_logits<SLAB_MIN, 256>), dim3(slabs, a.n), dim3(256), 0, s, a);
     if (a.next) hipLaunchKernelGGL(k_logits_pick, dim3(a.n), dim3(64), 0, s, a, slabs);
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }
