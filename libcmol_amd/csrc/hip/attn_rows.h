@@ -692,11 +692,11 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
 int launch_attn_window(const RowsArgs &a, hipStream_t s);
 int launch_attn_window_prompt(const RowsArgs &a, hipStream_t s);
 int launch_attn_shared(const RowsArgs &a, hipStream_t s);
-int launch_prompt_parts(const RowsArgs &a, hipStream_t s);   // merge of a prompt's parts (a.parts > 1)
 
-// Prompts whose query rows share the positions through LDS (attn_wprompt.hip).
-bool wprompt_takes(int n, int n_heads, int n_kv, int d_head);
-int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16);
+// Prompts whose query rows share the positions through LDS (attn_wprompt.hip),
+// WP_ROWS per work-group; d_head 64 and 128.
+constexpr int WP_ROWS = 128;
+bool wprompt_takes(int d_head);
 size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window, int sinks);
 int launch_wprompt(const RowsArgs &a, hipStream_t s);
 

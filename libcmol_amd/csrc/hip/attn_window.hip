@@ -63,19 +63,20 @@ __global__ __launch_bounds__(256) void k_window_merge(RowsArgs a)
 // ---- prompts ---------------------------------------------------------------------
 
 // Rows of a kv head are (token, head of the group), token-major, in blocks of
-// 16 RT; work-group (block and kv head, part) walks its part of the tiles that the
+// 16; work-group (block and kv head, part) walks its part of the tiles that the
 // block's tokens see between them.
-template <int DH, typename KT, int RT>
-__global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
+template <int DH, typename KT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window_prompt(RowsArgs a)
 {
 #pragma clang fp contract(off)
     constexpr int TP = rw_tp<KT>(), NW = 4;
     __shared__ RowsMeet<DH, NW> meet;
     __shared__ int odd;
-    const int G = a.n_heads / a.n_kv, rows = a.n * G;
-    const int kvh = blockIdx.x % a.n_kv, r0 = blockIdx.x / a.n_kv * 16 * RT, part = blockIdx.y;
+    const int G = a.n_heads / a.n_kv, rows = a.n * G, blocks = gridDim.x / a.n_kv;
+    // the blocks of the longest lines first
+    const int kvh = blockIdx.x % a.n_kv, r0 = (blocks - 1 - (int)(blockIdx.x / a.n_kv)) * 16, part = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int nr = min(16 * RT, rows - r0);
+    const int nr = min(16, rows - r0);
     RowsSeen seen;
     seen.first = a.pos0 + r0 / G;
     seen.last = a.pos0 + (r0 + nr - 1) / G;
@@ -84,21 +85,19 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     const RowsLine<TP> line = rows_line<TP>(seen.first, seen.last, a.window, a.sinks);
     const int T = line.tiles(), R = (T + a.parts - 1) / a.parts;
     const int u0 = min(part * R, T), u1 = min(u0 + R, T);
-    int pos[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) pos[rt] = a.pos0 + min(r0 + 16 * rt + (lane & 15), rows - 1) / G;
-    seen.pos = pos;
+    const int pos = a.pos0 + min(r0 + (lane & 15), rows - 1) / G;
+    seen.pos = &pos;
     auto row_at = [&](int r) {   // of q and out
         r = min(r0 + r, rows - 1);
         return (size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G;
     };
     const size_t base = (size_t)kvh * a.max_ctx * DH;
     const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
-    RowsWave<DH, KT, RT> w;
+    RowsWave<DH, KT, 1> w;
     w.load([&](int r) { return a.q + row_at(r) * DH; });
     if (tid == 0) odd = 0;
     __syncthreads();
-    rows_walk<DH, KT, RT, true>(w, k, v, line, u0 + wid, u1, NW, &seen);
+    rows_walk<DH, KT, 1, true>(w, k, v, line, u0 + wid, u1, NW, &seen);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
     bool bad = false;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
@@ -159,6 +158,23 @@ __global__ __launch_bounds__(256) void k_window_prompt(RowsArgs a)
     }
 }
 
+// The parts of (query head, token) rows, a lane per four dimensions.
+template <int DH>
+__global__ __launch_bounds__(256) void k_prompt_parts(RowsArgs a)
+{
+    constexpr int LPR = DH / 4;
+    const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;   // of out
+    if (row >= (size_t)a.n * a.n_heads) return;
+    const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
+    const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
+    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
+        *m = a.xm + x0 + j;
+        *l = a.xl + x0 + j;
+        *x = a.xo + (x0 + j) * DH;
+    });
+    *(f32x4 *)(a.out + row * DH + 4 * d4) = o;
+}
+
 // ---- plans and launches ------------------------------------------------------------
 
 // Most tiles of a token's line.
@@ -188,29 +204,59 @@ RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window,
     return p;
 }
 
-static int prompt_tiles(int n, int G) { return (long)n * G <= 16 ? 1 : (long)n * G <= 32 ? 2 : 4; }
-static int prompt_rt(int n, int G, int d_head, int kv_f16)
+// A prompt's form and the parts of its positions by what they are estimated to
+// cost, in microseconds: work-groups of 16 rows that read the cache themselves
+// (k_window_prompt), or of 128 that share it through LDS (attn_wprompt.hip).
+// Fitted to prompts of 16 .. 4096 tokens of 16/4 heads of 128 and 15/5 of 64
+// behind 5000 positions, windows of 128 .. 2048: the start and end of a
+// work-group, a tile's step (the matrix and vector instructions of the
+// work-groups that share a CU add up), the merge's launch and traffic.  Both
+// sides measured: 256 tokens, window 2048, fp16: 30 us by itself, 36 shared; 700:
+// 63, 46; 64 tokens, fp32: 24, 36; 500: 84, 51.
+struct PromptForm {
+    bool lds = false;
+    int parts = 1;
+    double us = 0;
+};
+static PromptForm prompt_form(bool lds, int n, int n_heads, int n_kv, int d_head, long ctx, int window, int sinks, int kv_f16)
 {
-    return std::min(prompt_tiles(n, G), d_head == 256 ? 1 : kv_f16 && d_head < 128 ? 4 : 2);
+    const int G = n_heads / n_kv, rows = lds ? WP_ROWS : 16, tp = lds || kv_f16 ? 32 : 16;
+    const long blocks = (long)n_kv * ceil_div((long)n * G, rows);
+    const long seen = std::min(ctx, std::min((long)window, ctx) + std::min((long)sinks, ctx) + std::min(n, rows / G + 1));
+    const long tiles = ceil_div(seen, tp) + 1;
+    const double dh = std::max(d_head, 32) / 128.0, traffic = (double)n * n_heads * d_head * 8 / 5e6;
+    double fixed = 0;
+    if (lds && !kv_f16) fixed = 4 + (double)std::min(ctx, (long)window + sinks + n) * n_kv * d_head * 16 / 4e6;   // the split copy
+    PromptForm best;
+    for (int p = 1; p <= 16 && p <= tiles; p++) {
+        const double wgs = (double)blocks * p, deep = ceil_div(blocks * p, 256);   // (of the fullest CU)
+        double us = fixed + (p > 1 ? 4.0 + p * traffic : 0.0);
+        if (lds) us += 8.0 * std::max(1.0, wgs / 512) + ceil_div(tiles, p) * (kv_f16 ? 1.0 : 1.55) * std::max(0.5 + 0.6 * dh, (0.16 + 0.64 * dh) * deep);
+        else us += 6.0 * std::max(1.0, wgs / 1024) + ceil_div(ceil_div(tiles, p), 4) * (kv_f16 ? 0.15 + 0.95 * dh : 0.25 + dh) * deep;
+        if (p == 1 || us < best.us) {
+            best.parts = p;
+            best.us = us;
+        }
+    }
+    best.lds = lds;
+    return best;
 }
-
-static int prompt_parts(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks, int rt)
+static PromptForm prompt_best(int n, int n_heads, int n_kv, int d_head, long ctx, int window, int sinks, int kv_f16)
 {
-    const int G = n_heads / n_kv;
-    const long blocks = (long)n_kv * ceil_div((long)n * G, 16 * rt);
-    const long span = std::min(span_tiles(max_ctx, window, sinks) + ceil_div(16 * rt, G * RW_PLAN_TP) + 1, (long)ceil_div(max_ctx, RW_PLAN_TP) + 2);
-    return (int)std::max(1L, std::min(RW_WGS / blocks, (long)ceil_div(span, 8)));
+    const PromptForm a = prompt_form(false, n, n_heads, n_kv, d_head, ctx, window, sinks, kv_f16);
+    if (!wprompt_takes(d_head)) return a;
+    const PromptForm b = prompt_form(true, n, n_heads, n_kv, d_head, ctx, window, sinks, kv_f16);
+    return b.us < a.us ? b : a;
 }
 
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
 {
     RowsPlan p;
-    const int G = n_heads / n_kv;
-    const bool lds = wprompt_takes(n, n_heads, n_kv, d_head);
-    for (int f16 = 0; f16 < 2; f16++)
-        p.parts = std::max(p.parts, lds ? wprompt_parts(n, n_heads, n_kv, d_head, max_ctx, window, sinks, f16)
-                                        : prompt_parts(n, n_heads, n_kv, max_ctx, window, sinks, prompt_rt(n, G, d_head, f16)));
-    if (lds) p.split = wprompt_split_bytes(n, n_kv, d_head, max_ctx, window, sinks);
+    for (int f16 = 0; f16 < 2; f16++) {
+        const PromptForm f = prompt_best(n, n_heads, n_kv, d_head, max_ctx, window, sinks, f16);
+        p.parts = std::max(p.parts, f.parts);
+        if (f.lds && !f16) p.split = wprompt_split_bytes(n, n_kv, d_head, max_ctx, window, sinks);
+    }
     if (p.parts > 1) p.cross = (size_t)n * n_heads * p.parts;
     return p;
 }
@@ -243,20 +289,27 @@ int launch_attn_window(const RowsArgs &a, hipStream_t s)
 int launch_attn_window_prompt(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
-    if (wprompt_takes(a.n, a.n_heads, a.n_kv, a.d_head)) return launch_wprompt(a, s);
-    const int G = a.n_heads / a.n_kv, rt = prompt_rt(a.n, G, a.d_head, a.kv_f16);
-    a.parts = std::min(a.parts, prompt_parts(a.n, a.n_heads, a.n_kv, a.max_ctx, a.window, a.sinks, rt));
-    const dim3 grid(a.n_kv * ceil_div((long)a.n * G, 16 * rt), a.parts), block(256);
-#define LAUNCH(DH, KT, RT) hipLaunchKernelGGL((k_window_prompt<DH, KT, RT>), grid, block, 0, s, a)
-#define PRO(DH)                                                                  \
-    if (rt == 1) { if (a.kv_f16) LAUNCH(DH, _Float16, 1); else LAUNCH(DH, float, 1); }  \
-    else if constexpr (DH < 256) {                                               \
-        if (a.kv_f16) { if (rt == 2) LAUNCH(DH, _Float16, 2); else LAUNCH(DH, _Float16, 4); }  \
-        else LAUNCH(DH, float, 2);                                               \
-    }
-    RW_BY_D_HEAD(a.d_head, PRO)
+    // (what this position's tokens see may be less than the plan's most: within its room)
+    PromptForm f = prompt_best(a.n, a.n_heads, a.n_kv, a.d_head, a.pos0 + a.n, a.window, a.sinks, a.kv_f16);
+    if (f.lds && !a.kv_f16 && !a.split)
+        f = prompt_form(false, a.n, a.n_heads, a.n_kv, a.d_head, a.pos0 + a.n, a.window, a.sinks, a.kv_f16);
+    a.parts = std::min(a.parts, f.parts);
+    if (f.lds) {
+        const int rc = launch_wprompt(a, s);
+        if (rc) return rc;
+    } else {
+        const dim3 grid(a.n_kv * ceil_div((long)a.n * (a.n_heads / a.n_kv), 16), a.parts), block(256);
+#define PRO(DH)                                                                                  \
+    if (a.kv_f16) hipLaunchKernelGGL((k_window_prompt<DH, _Float16>), grid, block, 0, s, a);     \
+    else hipLaunchKernelGGL((k_window_prompt<DH, float>), grid, block, 0, s, a);
+        RW_BY_D_HEAD(a.d_head, PRO)
 #undef PRO
-#undef LAUNCH
-    if (a.parts > 1 && launch_prompt_parts(a, s)) return -4;
+    }
+    if (a.parts > 1) {
+        const dim3 grid((unsigned)(((size_t)a.n * a.n_heads * a.d_head + 1023) / 1024)), block(256);
+#define MERGE(DH) hipLaunchKernelGGL(k_prompt_parts<DH>, grid, block, 0, s, a);
+        RW_BY_D_HEAD(a.d_head, MERGE)
+#undef MERGE
+    }
     return hipGetLastError() == hipSuccess ? 0 : -4;
 }

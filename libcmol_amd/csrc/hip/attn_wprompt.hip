@@ -25,7 +25,7 @@
 #include "attn_rows.h"
 #include "lds_limit.h"
 
-constexpr int WP_NT = 256, WP_ROWS = 128, WP_TP = 32;   // threads, rows, positions of a tile
+constexpr int WP_NT = 256, WP_TP = 32;   // threads, positions of a tile
 
 // Tiles of TP positions that a prompt's tokens see: `ns` of sinks, then the
 // run from lo (where the sinks reach into it, one run from 0).
@@ -535,59 +535,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     }
 }
 
-// The parts of (query head, token) rows, a lane per four dimensions.
-template <int DH>
-__global__ __launch_bounds__(256) void k_prompt_parts(RowsArgs a)
-{
-    constexpr int LPR = DH / 4;
-    const size_t row = (size_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;   // of out
-    if (row >= (size_t)a.n * a.n_heads) return;
-    const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
-    const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
-    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
-        *m = a.xm + x0 + j;
-        *l = a.xl + x0 + j;
-        *x = a.xo + (x0 + j) * DH;
-    });
-    *(f32x4 *)(a.out + row * DH + 4 * d4) = o;
-}
-
-int launch_prompt_parts(const RowsArgs &a, hipStream_t s)
-{
-    const dim3 grid((unsigned)(((size_t)a.n * a.n_heads * a.d_head + 1023) / 1024)), block(256);
-#define MERGE(DH) hipLaunchKernelGGL(k_prompt_parts<DH>, grid, block, 0, s, a);
-    RW_BY_D_HEAD(a.d_head, MERGE)
-#undef MERGE
-    return 0;
-}
-
-bool wprompt_takes(int n, int n_heads, int n_kv, int d_head)
-{
-    return (d_head == 64 || d_head == 128) && (long)n * (n_heads / n_kv) >= 64;
-}
-
-// Parts of the positions: what the rounds of two work-groups per CU and the
-// merge's traffic cost together, in microseconds (a tile and the start of a
-// work-group as they take at two per CU).
-int wprompt_parts(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16)
-{
-    const int G = n_heads / n_kv;
-    const long blocks = (long)n_kv * ceil_div((long)n * G, WP_ROWS);
-    const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + std::min(n, WP_ROWS / G + 1));
-    const long tiles = ceil_div(seen, WP_TP) + 1;
-    const double step = (kv_f16 ? 1.4 : 2.0) * d_head / 128;
-    int best = 1;
-    double least = 0;
-    for (int p = 1; p <= 16 && p <= tiles; p++) {
-        const double merge = p > 1 ? 4.0 + p * (double)n * n_heads * d_head * 8 / 5e6 : 0.0;
-        const double cost = ceil_div(blocks * p, RW_WGS) * (ceil_div(tiles, p) * step + 8.0) + merge;
-        if (p == 1 || cost < least) {
-            best = p;
-            least = cost;
-        }
-    }
-    return best;
-}
+bool wprompt_takes(int d_head) { return d_head == 64 || d_head == 128; }
 
 // Bytes of the split copy: the tiles, and their exponents behind them.
 size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window, int sinks)
@@ -623,13 +571,8 @@ static int launch_dh(const RowsArgs &a, hipStream_t s)
     return 0;
 }
 
-int launch_wprompt(const RowsArgs &a0, hipStream_t s)
+int launch_wprompt(const RowsArgs &a, hipStream_t s)
 {
-    RowsArgs a = a0;
-    a.parts = std::min(a.parts, wprompt_parts(a.n, a.n_heads, a.n_kv, a.d_head, a.max_ctx, a.window, a.sinks, a.kv_f16));
-    int rc;
-    if (a.kv_f16) rc = a.d_head == 128 ? launch_dh<128, true>(a, s) : launch_dh<64, true>(a, s);
-    else rc = a.d_head == 128 ? launch_dh<128, false>(a, s) : launch_dh<64, false>(a, s);
-    if (!rc && a.parts > 1) rc = launch_prompt_parts(a, s);
-    return rc ? rc : hipGetLastError() == hipSuccess ? 0 : -4;
+    if (a.kv_f16) return a.d_head == 128 ? launch_dh<128, true>(a, s) : launch_dh<64, true>(a, s);
+    return a.d_head == 128 ? launch_dh<128, false>(a, s) : launch_dh<64, false>(a, s);
 }

@@ -660,7 +660,7 @@ bool rows_args(RowsArgs &a, cmolhip_ctx_t *c, int n, const float *q, const void 
     a.kv_f16 = kv_f16 != 0;
     a.bal = p.bal;
     a.parts = p.parts;
-    a.split = ws;
+    a.split = p.split ? ws : nullptr;
     a.po = (float *)((uint8_t *)ws + align_up(p.split, ALIGN));
     a.xo = a.po + p.pieces * d_head;
     a.pm = a.xo + p.cross * d_head;
