@@ -171,7 +171,9 @@ int cmolhip_attn_decode(cmolhip_ctx_t *c, int n, const float *q,
  * n_kv * max_ctx * d_head, else a multiple of 8 that is no smaller) and is
  * [n_kv][max_ctx][d_head]; query head h reads kv head h / (n_heads / n_kv).
  * seqlen[n] (device int32) is the number of positions in the cache, the
- * token's own among them, taken as max_ctx where it is above.  Scores are
+ * token's own among them, taken as max_ctx where it is above.  max_ctx and a
+ * prefix are at most 2^30 positions, a call at most 2^23 query rows
+ * (n * n_heads).  Scores are
  * q . k / sqrt(d_head); a row that sees no position (a length of 0 or below, a
  * slot below 0: padding of a batch) is 0.  Positions a row does not see do not
  * reach it whatever they hold.  Sums and softmax statistics are fp32. */

@@ -118,15 +118,19 @@ static int shared_rt(int n, int G, int d_head, int kv_f16)
     return (long)n * G <= 16 || d_head == 256 || !kv_f16 ? 1 : 2;
 }
 
-// Work-groups of the prefix to aim for: with those of the own positions one
-// round of two per CU (32 sessions of 4 heads behind 8192 positions, fp16: 24.6
-// us at 96, 20.5 at 160, 23.5 at 224, 26.4 at 512).
-constexpr int SH_PREFIX_WGS = 192;
-
-static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt)
+// Parts of the prefix.  Its work-groups and those of the own positions make one
+// round of two per CU at 192 (32 sessions of 4 heads behind 8192 positions, fp16,
+// in the kernel: 24.6 us at 96, 20.5 at 160, 21.2 at 192, 23.5 at 224, 26.4 at
+// 512).  Where a wave then has more than twenty tiles to walk the prefix takes
+// most of two per CU (65536 positions: 84 us at 192, 71 at 448; 16000 over fp32,
+// 48 sessions: 103, 81; 320, which gives every fourth CU a second one, lies
+// between).
+static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt, int kv_f16)
 {
     const long blocks = (long)n_kv * ceil_div((long)n * (n_heads / n_kv), 16 * rt);
-    return (int)std::max(1L, std::min(SH_PREFIX_WGS / blocks, (long)ceil_div(ceil_div(prefix, RW_PLAN_TP), SH_NW)));
+    const long tiles = ceil_div(prefix, kv_f16 ? 32 : 16);
+    const long wgs = tiles * blocks > 20L * SH_NW * 192 ? 448 : 192;
+    return (int)std::max(1L, std::min(wgs / blocks, (tiles + SH_NW - 1) / SH_NW));
 }
 
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
@@ -135,7 +139,7 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
     const int G = n_heads / n_kv;
     p.parts = 1;
     for (int f16 = 0; f16 < 2; f16++)
-        p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16)));
+        p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16), f16));
     p.cross = prefix ? (size_t)n * n_heads * p.parts : 0;
     p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP), 8);
     p.pieces = (size_t)n_kv * (p.bal + n) * G;
@@ -146,10 +150,8 @@ int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
     const int G = a.n_heads / a.n_kv, rt = shared_rt(a.n, G, a.d_head, a.kv_f16);
-    a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt));
-    const size_t wgs = shared_prefix_wgs(a, rt) + (size_t)a.n_kv * ceil_div(G, 16) * (a.bal + a.n);
-    if (wgs > INT32_MAX) return -6;
-    const dim3 grid((unsigned)wgs), block(256);
+    a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt, a.kv_f16));
+    const dim3 grid(shared_prefix_wgs(a, rt) + (unsigned)(a.n_kv * ceil_div(G, 16)) * (a.bal + a.n)), block(256);
 #define SHA(DH)                                                                                          \
     if (!a.kv_f16) hipLaunchKernelGGL((k_shared<DH, float, 1>), grid, block, 0, s, a);                   \
     else if (DH == 256 || rt == 1) hipLaunchKernelGGL((k_shared<DH, _Float16, 1>), grid, block, 0, s, a); \

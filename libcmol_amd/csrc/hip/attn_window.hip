@@ -2,6 +2,8 @@
 // single tokens of many sessions, and consecutive tokens of one.
 #include "attn_rows.h"
 
+#include <cstdlib>
+
 // ---- single tokens ---------------------------------------------------------------
 
 // Work-group of NW waves (16 query heads of a kv head, slot): the piece of that
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
 #pragma clang fp contract(off)
     constexpr int TP = rw_tp<KT>(), NW = 4;
     __shared__ RowsMeet<DH, NW> meet;
-    __shared__ int odd;
+    __shared__ int odd, odd_row[16];
     const int G = a.n_heads / a.n_kv, rows = a.n * G, blocks = gridDim.x / a.n_kv;
     // the blocks of the longest lines first
     const int kvh = blockIdx.x % a.n_kv, r0 = (blocks - 1 - (int)(blockIdx.x / a.n_kv)) * 16, part = blockIdx.y;
@@ -96,15 +98,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
     RowsWave<DH, KT, 1> w;
     w.load([&](int r) { return a.q + row_at(r) * DH; });
     if (tid == 0) odd = 0;
+    if (tid < 16) odd_row[tid] = 0;
     __syncthreads();
     rows_walk<DH, KT, 1, true>(w, k, v, line, u0 + wid, u1, NW, &seen);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
-    bool bad = false;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         if (r >= nr) return;
-        float z = 0.0f;
+        float z = l * 0.0f;
         for (auto &y : x) z += y * 0.0f;
-        bad |= !(z == 0.0f);
+        if (!(z == 0.0f)) odd = odd_row[r] = 1;
         if (a.parts == 1) {
             const float f = 1.0f / l;
             for (auto &y : x) y *= f;
@@ -119,14 +121,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
         }
     });
     // A masked position is in its tile's products with weight 0, which a V row
-    // that is not finite turns into NaN for the rows that do not see it: where
-    // an output is not finite, the block's rows are walked again one by one.
-    if (bad) odd = 1;
+    // that is not finite turns into NaN for the rows that do not see it: rows
+    // whose outputs are not finite are walked again one by one.
     __syncthreads();
     if (!odd) return;
     constexpr int DL = RowState<DH>::DL;
     const bool on = lane * DL < DH;
     for (int r = wid; r < nr; r += NW) {
+        if (!odd_row[r]) continue;
         const size_t qa = row_at(r) * DH + (on ? lane * DL : 0);
         const int p = a.pos0 + (r0 + r) / G;
         RowState<DH> t;
@@ -241,12 +243,14 @@ static PromptForm prompt_form(bool lds, int n, int n_heads, int n_kv, int d_head
     best.lds = lds;
     return best;
 }
+// (CMOL_WINDOW_PROMPT=0 / 1: the first form / the second wherever it runs)
 static PromptForm prompt_best(int n, int n_heads, int n_kv, int d_head, long ctx, int window, int sinks, int kv_f16)
 {
     const PromptForm a = prompt_form(false, n, n_heads, n_kv, d_head, ctx, window, sinks, kv_f16);
-    if (!wprompt_takes(d_head)) return a;
+    const char *e = getenv("CMOL_WINDOW_PROMPT");
+    if (!wprompt_takes(d_head) || (e && e[0] == '0')) return a;
     const PromptForm b = prompt_form(true, n, n_heads, n_kv, d_head, ctx, window, sinks, kv_f16);
-    return b.us < a.us ? b : a;
+    return b.us < a.us || (e && e[0] == '1') ? b : a;
 }
 
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
@@ -289,15 +293,17 @@ int launch_attn_window(const RowsArgs &a, hipStream_t s)
 int launch_attn_window_prompt(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
+    const int room = a.parts, seen = a.pos0 + a.n;
     // (what this position's tokens see may be less than the plan's most: within its room)
-    PromptForm f = prompt_best(a.n, a.n_heads, a.n_kv, a.d_head, a.pos0 + a.n, a.window, a.sinks, a.kv_f16);
-    if (f.lds && !a.kv_f16 && !a.split)
-        f = prompt_form(false, a.n, a.n_heads, a.n_kv, a.d_head, a.pos0 + a.n, a.window, a.sinks, a.kv_f16);
-    a.parts = std::min(a.parts, f.parts);
+    PromptForm f = prompt_best(a.n, a.n_heads, a.n_kv, a.d_head, seen, a.window, a.sinks, a.kv_f16);
     if (f.lds) {
-        const int rc = launch_wprompt(a, s);
-        if (rc) return rc;
-    } else {
+        a.parts = std::min(room, f.parts);
+        // no room for the f16 pairs, or a refused LDS limit: the other form
+        if ((!a.kv_f16 && !a.split) || launch_wprompt(a, s))
+            f = prompt_form(false, a.n, a.n_heads, a.n_kv, a.d_head, seen, a.window, a.sinks, a.kv_f16);
+    }
+    if (!f.lds) {
+        a.parts = std::min(room, f.parts);
         const dim3 grid(a.n_kv * ceil_div((long)a.n * (a.n_heads / a.n_kv), 16), a.parts), block(256);
 #define PRO(DH)                                                                                  \
     if (a.kv_f16) hipLaunchKernelGGL((k_window_prompt<DH, _Float16>), grid, block, 0, s, a);     \

@@ -135,7 +135,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     constexpr int RPP = 1024 / (2 * DH);              // fp16: V rows per 1 KiB piece
     constexpr int VPW = TP / RPP / 4;                 // fp16: V pieces per wave
     extern __shared__ __attribute__((aligned(256))) uint8_t smem_w[];   // K [stage][KB], V the same
-    __shared__ int odd;
+    __shared__ int odd, odd_row[WP_ROWS];
 
     const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, col = lane & 15;
     const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -471,7 +471,9 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     }
 
     // ---- outputs: lane (col, g) holds dimensions 16d + 4g + i of row col
-    bool bad = false;
+    if (tid == 0) odd = 0;
+    if (tid < WP_ROWS) odd_row[tid] = 0;
+    __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         float ls = l[rt];
@@ -494,18 +496,16 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
             a.xm[at] = m[rt] == -INFINITY ? -INFINITY : -mk[rt];   // of the weights as they are
             a.xl[at] = ls;
         }
-        bad |= valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f);
+        if (valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f)) odd = odd_row[r] = 1;
     }
     // A masked position is in its tile's products with weight 0, which a V row
-    // that is not finite turns into NaN for the rows that do not see it: where
-    // an output is not finite, the block's rows are walked again one by one.
-    if (tid == 0) odd = 0;
-    __syncthreads();
-    if (bad) odd = 1;
+    // that is not finite turns into NaN for the rows that do not see it: rows
+    // whose outputs are not finite are walked again one by one.
     __syncthreads();
     if (!odd) return;
     constexpr int DL = RowState<DH>::DL;
     for (int r = wid; r < nr; r += WP_NT / 64) {
+        if (!odd_row[r]) continue;
         const size_t qa = row_at(r) * DH + lane * DL;
         const int p = a.pos0 + (r0 + r) / G;
         RowState<DH> s;

@@ -588,14 +588,18 @@ struct OnDevice {
     }
 };
 
+// positions of a cache or prefix; query rows of a call
+constexpr int ROWS_MAX_CTX = 1 << 30;
+constexpr size_t ROWS_MAX = (size_t)1 << 23;
+
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 // Shapes the rows kernels take: a workspace size, or 0 for a refusal (*rc).
 bool rows_shape(int n, int n_heads, int n_kv, int d_head, int max_ctx, int *rc)
 {
     *rc = E_ARGS;
-    if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_kv > 65535 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
-    if (d_head < 1 || (size_t)n_heads * d_head > INT32_MAX || (size_t)n * n_heads > INT32_MAX) return false;
+    if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
+    if (max_ctx > ROWS_MAX_CTX || (size_t)n * n_heads > ROWS_MAX || d_head < 1) return false;
     *rc = E_UNSUPPORTED;
     if (d_head != 16 && d_head != 32 && d_head != 64 && d_head != 128 && d_head != 256) return false;
     *rc = E_OK;
@@ -625,7 +629,7 @@ size_t window_bytes(bool prompt, int n, int n_heads, int n_kv, int d_head, int m
 size_t shared_bytes(int n, int n_heads, int n_kv, int d_head, int prefix_len, int max_ctx, RowsPlan *p, int *rc)
 {
     if (!rows_shape(n, n_heads, n_kv, d_head, max_ctx, rc)) return 0;
-    if (prefix_len < 0) {
+    if (prefix_len < 0 || prefix_len > ROWS_MAX_CTX) {
         *rc = E_ARGS;
         return 0;
     }

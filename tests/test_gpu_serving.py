@@ -113,6 +113,10 @@ WINDOW_CASES = [
     (8, 2, 64, 500, [500, 20, 499], 2**31 - 1, 2**31 - 1), (15, 5, 64, 2000, [2000, 64, 1000, 601, 602, 603], 601, 1),
     (2, 1, 128, 5000, [5000, 4999], 4000, 64), (1, 1, 64, 37, [37], 5, 0),
     (3, 3, 128, 64, [int(x) for x in np.random.default_rng(3).integers(0, 65, 70)], 20, 3),
+    # long contexts in balanced ranges: one item, more items than a wave has lanes, items of nothing among them
+    (2, 1, 64, 3000, [2999], 2500, 40), (4, 1, 64, 1500, [int(x) for x in np.random.default_rng(4).integers(-5, 1501, 100)], 1200, 4),
+    (6, 3, 128, 2100, [2100, 0, 1500, 3, 2099, 0], 1700, 100), (2, 2, 256, 1400, [1400, 700], 1300, 0),
+    (16, 2, 16, 1300, [1300, 1299, 64], 1100, 9), (8, 1, 32, 1300, [1300, 31], 1290, 5),
 ]
 
 
@@ -191,9 +195,20 @@ PROMPT_CASES = [
 ]
 
 
+def prompt_form(monkeypatch, form):
+    """The prompt's form: None the estimated one, "0" 16-row work-groups, "1"
+    128-row ones that share the positions through LDS."""
+    if form is None:
+        monkeypatch.delenv("CMOL_WINDOW_PROMPT", raising=False)
+    else:
+        monkeypatch.setenv("CMOL_WINDOW_PROMPT", form)
+
+
+@pytest.mark.parametrize("form", [None, "0", "1"])
 @pytest.mark.parametrize("f16", [F32, F16])
 @pytest.mark.parametrize("heads,kv,dh,n,pos0,max_ctx,window,sinks", PROMPT_CASES, ids=str)
-def test_prompt_against_64_bits(ctx, heads, kv, dh, n, pos0, max_ctx, window, sinks, f16):
+def test_prompt_against_64_bits(ctx, monkeypatch, heads, kv, dh, n, pos0, max_ctx, window, sinks, f16, form):
+    prompt_form(monkeypatch, form)
     c = native.Ctx(256 << 20)
     rng = np.random.default_rng(heads * dh + n)
     q = rng.standard_normal((n, heads, dh)).astype(np.float32)
@@ -209,11 +224,13 @@ def test_prompt_against_64_bits(ctx, heads, kv, dh, n, pos0, max_ctx, window, si
     c.close()
 
 
+@pytest.mark.parametrize("form", ["0", "1"])
 @pytest.mark.parametrize("f16", [F32, F16])
 @pytest.mark.parametrize("heads,kv,dh", [(16, 4, 128), (9, 3, 64), (4, 4, 32)])
-def test_prompt_positions_that_are_not_finite(ctx, heads, kv, dh, f16):
+def test_prompt_positions_that_are_not_finite(ctx, monkeypatch, heads, kv, dh, f16, form):
     """NaN and infinities in positions that some tokens see and others mask:
     the tokens that do not see one come out as without it."""
+    prompt_form(monkeypatch, form)
     n, pos0, max_ctx, window, sinks = 90, 40, 160, 30, 2
     rng = np.random.default_rng(2)
     q = rng.standard_normal((n, heads, dh)).astype(np.float32)
@@ -230,13 +247,15 @@ def test_prompt_positions_that_are_not_finite(ctx, heads, kv, dh, f16):
         close(got[i], want, tol, f"token {i}")
 
 
+@pytest.mark.parametrize("form", ["0", "1"])
 @pytest.mark.parametrize("dh", [64, 128])
 @pytest.mark.parametrize("k_scale,v_scale", [(1e-6, 1e-6), (1e-3, 1e9), (1e-30, 1e-30), (1e3, 1.0), (1.0, 1e30)])
-def test_prompt_over_caches_of_any_range(ctx, dh, k_scale, v_scale):
+def test_prompt_over_caches_of_any_range(ctx, monkeypatch, dh, k_scale, v_scale, form):
     """fp32 caches far from 1, each position's row times another power of ten
     up to 10^4; the queries make up for K, so the scores are ordinary.  The
     absolute term: a value of a tile of 32 positions is held to 2^-33 of the
     tile's largest."""
+    prompt_form(monkeypatch, form)
     heads, kv, n, pos0, max_ctx, window, sinks = 8, 2, 70, 100, 200, 90, 5
     rng = np.random.default_rng(int(dh + np.log10(v_scale)))
     q = (rng.standard_normal((n, heads, dh)) / k_scale / 1e3).astype(np.float32)
@@ -285,6 +304,11 @@ SHARED_CASES = [
     (32, 1, 64, 95, 96, [33, 2, 64], 64), (20, 2, 128, 64, 64, [5000, 12], 31), (34, 2, 32, 31, 40, [5, 6], 8),
     (15, 5, 64, 513, 600, [int(x) for x in np.random.default_rng(5).integers(0, 90, 70)], 90),
     (2, 1, 64, 5000, 5000, [1, 700], 700), (1, 1, 128, 33, 33, [0], 4), (8, 8, 64, 200, 256, [10, 20, 30], 40),
+    # own contexts in balanced ranges, more sessions than a wave has lanes
+    (4, 2, 64, 300, 300, [int(x) for x in np.random.default_rng(6).integers(-5, 400, 100)], 400),
+    (16, 4, 128, 100, 128, [900, 0, 31, 899], 900), (4, 2, 256, 70, 70, [600, 3, 0], 600),
+    # a long prefix before a few rows: many parts
+    (4, 1, 64, 9000, 9000, [3, 0], 16), (2, 1, 16, 20000, 20000, [40], 64),
 ]
 
 
@@ -420,6 +444,26 @@ def test_logits_against_the_host(ctx, n, V, inplace):
         assert nxt[i] == best, f"row {i}"
 
 
+@pytest.mark.parametrize("n", [2, 17])
+def test_logits_of_words_repeated_often(ctx, n):
+    """1 to 500 occurrences of a word, penalties from 1 + 2^-23 to 1e9: bit for
+    bit the host's, one division or product after the other; few and many rows
+    (small and large slabs)."""
+    V = 140000
+    rng = np.random.default_rng(n)
+    x = (10.0 ** rng.uniform(-40, 30, (n, V)) * rng.choice([-1, 1], (n, V))).astype(np.float32)
+    x[:, :2000] = (5 * rng.standard_normal((n, 2000))).astype(np.float32)
+    ids = rng.permutation(2000)[:40].tolist() + rng.integers(0, V, 20).tolist()
+    counts = rng.integers(1, 500, 60)
+    hist = [rng.permutation(np.repeat(ids, counts)).tolist() for _ in range(n)]
+    rep = [[1.1, 1.0 + 2.0**-23, 1.5, 2.0, 16.0, 1e9, 1.0001, np.float32(2) - np.float32(2.0**-23)][i % 8] for i in range(n)]
+    got, nxt = logits_call(ctx, x, hist=hist, rep=rep)
+    for i in range(n):
+        want, best = logits_reference(x[i], hist[i], rep[i], 0, 0, [], None)
+        assert np.array_equal(got[i].view(np.uint32), want.view(np.uint32)), f"row {i}"
+        assert nxt[i] == best, f"row {i}"
+
+
 def test_logits_edges(ctx):
     """A row without an allowed token, ties, infinities and NaN, a token
     repeated past every range, an id listed twice, empty lists."""
@@ -482,7 +526,7 @@ def test_refusals(ctx):
 
     for f in (win, pro, sha):
         for bad in (dict(c=None), dict(n=0), dict(n=65536), dict(q=None), dict(k=None), dict(v=None), dict(o=None),
-                    dict(heads=3), dict(kv=0), dict(ctx_=0), dict(ws_=None), dict(size=0), dict(q=d + 4), dict(k=d + 2),
+                    dict(heads=3), dict(kv=0), dict(ctx_=0), dict(ctx_=(1 << 30) + 1), dict(ws_=None), dict(size=0), dict(q=d + 4), dict(k=d + 2),
                     dict(v=d + 8), dict(ws_=d + 4), dict(o=out + 4)):
             assert f(**bad) == A, (f.__name__, bad)
         assert f(dh=48) == native.CMOL_ERR_UNSUPPORTED

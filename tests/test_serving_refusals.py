@@ -15,7 +15,8 @@ def window(n=2, heads=4, kv=2, dh=64, ctx=100, window=16, sinks=2):
 
 
 BAD_SHAPES = [dict(n=0), dict(n=-1), dict(n=65536), dict(heads=0), dict(heads=3), dict(heads=1), dict(kv=0), dict(kv=-2),
-              dict(dh=0), dict(dh=-64), dict(dh=48), dict(dh=8), dict(dh=512), dict(ctx=0), dict(ctx=-5)]
+              dict(dh=0), dict(dh=-64), dict(dh=48), dict(dh=8), dict(dh=512), dict(ctx=0), dict(ctx=-5), dict(ctx=(1 << 30) + 1),
+              dict(n=65535, heads=256)]
 
 
 @pytest.mark.parametrize("bad", BAD_SHAPES + [dict(window=0), dict(window=-1), dict(sinks=-1)], ids=str)
@@ -33,6 +34,7 @@ def test_shared_bytes_refuse(bad):
     assert f(*args.values()) > 0
     assert f(*{**args, **bad}.values()) == 0
     assert f(2, 4, 2, 64, -1, 100) == 0
+    assert f(2, 4, 2, 64, (1 << 30) + 1, 100) == 0
     assert f(2, 4, 2, 64, 0, 100) > 0
 
 
