@@ -173,10 +173,12 @@ int cmolhip_attn_decode(cmolhip_ctx_t *c, int n, const float *q,
  * seqlen[n] (device int32) is the number of positions in the cache, the
  * token's own among them, taken as max_ctx where it is above.  max_ctx and a
  * prefix are at most 2^30 positions, a call at most 2^23 query rows
- * (n * n_heads).  Scores are
- * q . k / sqrt(d_head); a row that sees no position (a length of 0 or below, a
- * slot below 0: padding of a batch) is 0.  Positions a row does not see do not
- * reach it whatever they hold.  Sums and softmax statistics are fp32. */
+ * (n * n_heads) and 65535 kv heads.  Scores are q . k / sqrt(d_head); a row
+ * that sees no position (a length of 0 or below, a slot below 0: padding of a
+ * batch) is 0.  Positions a row does not see do not reach it whatever they
+ * hold.  Sums and softmax statistics are fp32; where values are carried as
+ * pairs of fp16 numbers they keep 22 bits, and 2^-33 of the largest of their
+ * query, K or V row. */
 
 /* Decode attention of n sessions (1..65535) over a sliding window with sinks:
  * a session of length L sees positions t < sinks and t >= L - window (window

@@ -598,7 +598,7 @@ bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 bool rows_shape(int n, int n_heads, int n_kv, int d_head, int max_ctx, int *rc)
 {
     *rc = E_ARGS;
-    if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
+    if (n < 1 || n > GEMM_MAX_N || n_kv < 1 || n_kv > 65535 || n_heads < n_kv || n_heads % n_kv || max_ctx < 1) return false;
     if (max_ctx > ROWS_MAX_CTX || (size_t)n * n_heads > ROWS_MAX || d_head < 1) return false;
     *rc = E_UNSUPPORTED;
     if (d_head != 16 && d_head != 32 && d_head != 64 && d_head != 128 && d_head != 256) return false;

@@ -44,6 +44,14 @@ def test_prompt_bytes_refuse_tokens_past_the_cache():
     assert f(*window(n=101)) == 0
 
 
+def test_bytes_refuse_more_kv_heads_than_a_grid_holds():
+    L = native.lib()
+    for kv, takes in ((65535, True), (65536, False)):
+        assert (L.cmolhip_attn_window_bytes(1, kv, kv, 16, 1, 1, 0) > 0) == takes
+        assert (L.cmolhip_attn_window_prompt_bytes(1, kv, kv, 64, 1, 1, 0) > 0) == takes
+        assert (L.cmolhip_attn_shared_bytes(1, kv, kv, 16, 1, 1) > 0) == takes
+
+
 def test_bytes_at_the_largest_arguments():
     """Sizes that pass 32 bits come out whole; a window or a sink count past
     the cache is the cache's length."""
