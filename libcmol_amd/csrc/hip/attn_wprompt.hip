@@ -13,10 +13,14 @@
 //     (ds_read_b64_tr_b16) of the second product.
 //   fp32 cache: k_prompt_split lays the positions the prompt sees out
 //     once per call as f16 pairs (x = hi + lo), both operands in their order.
-//     A tile is scaled by a power of two that puts its largest |K| (|V|) into
+//     A tile is scaled by powers of two that put its largest |K| and |V| into
 //     [2^9, 2^10), so hi and lo are normal f16 numbers whatever the cache's
-//     range: 22 bits of a value, 2^-33 of the tile's largest below.  The score
-//     takes K's exponent back into its exponential, the weights V's.
+//     range: 22 bits of a value, 2^-33 of the tile's largest below.  Where a
+//     position's largest is below 2^-12 of the tile's, every position of the
+//     tile is scaled by itself (`wide`): what a row does not see, or gives no
+//     weight, leaves no trace in what it sees.  The score takes K's exponent
+//     back; V's goes into the exponent of the weight, whose softmax reference
+//     then follows what reaches the output, and the weights' sum takes it out.
 // Products are exact (lo.lo, below 2^-22 of each, is left out over fp32), sums
 // fp32; the query is split as the walk's of attn_rows.h, the weights too.
 // A tile has 2 x 2 (fp32 3) products per (row tile, 16 positions, 32
@@ -41,7 +45,12 @@ struct PromptTiles {
     __host__ __device__ int count(int last, int tp) const { return ns + (last + tp - lo) / tp; }
 };
 
-// A split tile: K hi and lo pieces, V hi and lo pieces, WP_TP positions.
+// A split tile: K hi and lo pieces, V hi and lo pieces, WP_TP positions.  Its
+// exponents are K's, V's, whether it is wide and the least of V's; for a wide
+// one, K's and V's of each position less the tile's.
+constexpr int WP_HEAD = 4, WP_POS = 2 * WP_TP;   // ints of a tile: all heads first, then the positions'
+constexpr int WP_LEXP = 20;                      // the weights' sum is held in units of 2^20
+constexpr int WP_FAR = 90;                       // most that V's exponents may differ by
 template <int DH>
 constexpr int wp_tile_halves() { return WP_TP * DH * 4; }
 
@@ -50,7 +59,7 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
 {
 #pragma clang fp contract(off)
     constexpr int KS = DH / 32, DT = DH / 16, NK = 2 * KS * 64 / 256, NV = DT * 64 / 256, TH = wp_tile_halves<DH>();
-    __shared__ float top[2][4];
+    __shared__ float top[2][WP_TP];   // largest of each position's K, V
     const int tile = blockIdx.x, kvh = blockIdx.y, tid = threadIdx.x;
     const PromptTiles pt(a.pos0, a.window, a.sinks, WP_TP);
     const int p0 = tile < pt.ns ? tile * WP_TP : pt.lo + (tile - pt.ns) * WP_TP;
@@ -58,7 +67,7 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
     const size_t base = ((size_t)kvh * a.max_ctx + p0) * DH;
     const float *kb = (const float *)a.k + base, *vb = (const float *)a.v + base;
     dst += ((size_t)kvh * tiles + tile) * TH;
-    float k[NK][8], v[NV][8], tk = 0.0f, tv = 0.0f;
+    float k[NK][8], v[NV][8];
 #pragma unroll
     for (int j = 0; j < NK; j++) {
         const int it = tid + 256 * j, lane = it & 63, cs = it >> 6, c = cs / KS, s = cs % KS, p = 16 * c + (lane & 15);
@@ -66,10 +75,7 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
         for (int h = 0; h < 2; h++) {
             const f32x4 x = p < cnt ? *(const f32x4 *)(kb + (size_t)p * DH + 32 * s + 8 * (lane >> 4) + 4 * h) : f32x4{};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                k[j][4 * h + e] = x[e];
-                if (fabsf(x[e]) < INFINITY) tk = fmaxf(tk, fabsf(x[e]));
-            }
+            for (int e = 0; e < 4; e++) k[j][4 * h + e] = x[e];
         }
     }
 #pragma unroll
@@ -79,43 +85,79 @@ __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst,
         for (int e = 0; e < 8; e++) {
             const int p = (e < 4 ? 0 : 12) + 4 * g + e;
             v[j][e] = p < cnt ? vb[(size_t)p * DH + 16 * t + (lane & 15)] : 0.0f;
-            if (fabsf(v[j][e]) < INFINITY) tv = fmaxf(tv, fabsf(v[j][e]));
         }
     }
-    tk = wave_max(tk);
-    tv = wave_max(tv);
-    if ((tid & 63) == 0) {
-        top[0][tid >> 6] = tk;
-        top[1][tid >> 6] = tv;
+    {   // eight threads per position
+        const int p = tid >> 3;
+        float tk = 0.0f, tv = 0.0f;
+#pragma unroll
+        for (int j = 0; j < DH / 32; j++) {
+            const size_t at = (size_t)p * DH + 4 * ((tid & 7) + 8 * j);
+            const f32x4 x = p < cnt ? *(const f32x4 *)(kb + at) : f32x4{}, y = p < cnt ? *(const f32x4 *)(vb + at) : f32x4{};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (fabsf(x[e]) < INFINITY) tk = fmaxf(tk, fabsf(x[e]));
+                if (fabsf(y[e]) < INFINITY) tv = fmaxf(tv, fabsf(y[e]));
+            }
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+            tk = fmaxf(tk, __shfl_xor(tk, o, 64));
+            tv = fmaxf(tv, __shfl_xor(tv, o, 64));
+        }
+        if ((tid & 7) == 0) {
+            top[0][p] = tk;
+            top[1][p] = tv;
+        }
     }
     __syncthreads();
-    int ex[2];
+    // lanes 0 .. 31: K of a position, 32 .. 63: V (positions of zeros do not make a
+    // tile wide; theirs is an exponent that raises no reference of ordinary values)
+    auto exponent = [](float x) { return x > 0.0f ? max(ilogbf(x), -100) - 9 : -45; };
+    const int own = tid & 63;
+    const float mine = top[own >> 5][own & 31];
+    float most = mine, least = mine > 0.0f ? mine : INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float t = fmaxf(fmaxf(top[i][0], top[i][1]), fmaxf(top[i][2], top[i][3]));
-        ex[i] = t > 0.0f ? max(ilogbf(t), -100) - 9 : 0;
-        if (tid == 0) exps[((size_t)kvh * tiles + tile) * 2 + i] = ex[i];
+    for (int o = 16; o > 0; o >>= 1) {
+        most = fmaxf(most, __shfl_xor(most, o, 64));
+        least = fminf(least, __shfl_xor(least, o, 64));
     }
-    auto put = [&](const float (&x)[8], int e, _Float16 *at) {
+    const bool wide = __ballot(least < most * 0x1p-12f) != 0;
+    const int em = exponent(most), ex[2] = {__builtin_amdgcn_readlane(em, 0), __builtin_amdgcn_readlane(em, 32)};
+    const size_t at = (size_t)kvh * tiles + tile;
+    int low = wide && (own & 31) < cnt ? exponent(mine) : em;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor(low, o, 64));
+    low = __builtin_amdgcn_readlane(low, 32);
+    int *pos = exps + (size_t)a.n_kv * tiles * WP_HEAD + at * WP_POS;
+    if (tid < WP_POS) {
+        pos[tid] = wide ? exponent(mine) - em : 0;
+        if (tid < WP_HEAD) exps[at * WP_HEAD + tid] = tid == 0 ? ex[0] : tid == 1 ? ex[1] : tid == 2 ? wide : low;
+    }
+    auto scale = [&](int i, int p) { return wide ? exponent(top[i][p]) : ex[i]; };
+    auto put = [&](const float (&y)[8], _Float16 *to) {
         f16x8 hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float y = ldexpf(x[i], -e);
-            hi[i] = (_Float16)y;
-            lo[i] = (_Float16)(y - (float)hi[i]);
+            hi[i] = (_Float16)y[i];
+            lo[i] = (_Float16)(y[i] - (float)hi[i]);
         }
-        *(f16x8 *)at = hi;
-        *(f16x8 *)(at + 512) = lo;
+        *(f16x8 *)to = hi;
+        *(f16x8 *)(to + 512) = lo;
     };
 #pragma unroll
     for (int j = 0; j < NK; j++) {
-        const int it = tid + 256 * j;
-        put(k[j], ex[0], dst + (it >> 6) * 1024 + (it & 63) * 8);
+        const int it = tid + 256 * j, e = scale(0, 16 * ((it >> 6) / KS) + (it & 15));
+#pragma unroll
+        for (int i = 0; i < 8; i++) k[j][i] = ldexpf(k[j][i], -e);
+        put(k[j], dst + (it >> 6) * 1024 + (it & 63) * 8);
     }
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int it = tid + 256 * j;
-        put(v[j], ex[1], dst + TH / 2 + (it >> 6) * 1024 + (it & 63) * 8);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[j][i] = ldexpf(v[j][i], -scale(1, (i < 4 ? 0 : 12) + 4 * ((it & 63) >> 4) + i));
+        put(v[j], dst + TH / 2 + (it >> 6) * 1024 + (it & 63) * 8);
     }
 }
 
@@ -161,7 +203,8 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     const uint8_t *vbp = (const uint8_t *)uniform_ptr((const KT *)a.v + base);
     const uint8_t *sb = (const uint8_t *)uniform_ptr(split + (size_t)kvh * tiles * wp_tile_halves<DH>());
     typedef const __attribute__((address_space(4))) int cint;   // (scalar loads)
-    cint *ex = (cint *)uniform_ptr(exps + (size_t)kvh * tiles * 2);
+    cint *ex = (cint *)uniform_ptr(exps + (size_t)kvh * tiles * WP_HEAD);
+    const int *px = exps + (size_t)a.n_kv * tiles * WP_HEAD + (size_t)kvh * tiles * WP_POS;
     const int vrow = lane / (DH / 8), vch = lane % (DH / 8);
     uint8_t *const kl_ = smem_w, *const vl_ = smem_w + 2 * KB;
     auto issue_k = [&](int st, int u) {
@@ -252,18 +295,30 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
                 ql[rt][s][e] = (_Float16)(y - (float)qh[rt][s][e]);
             }
     }
-    // the largest exponent of V among the part's tiles: the outputs' unit
-    int ve = 0;
+    // V of so many magnitudes in the block's tiles (whatever the part) that a
+    // weight's sum could leave the range of fp32 beside another's contribution:
+    // every row one by one
+    bool far = false;
+    int most = 0;
     if constexpr (!F16) {
-        ve = -1000;
-        for (int u = u0 + lane; u < u1; u += 64) ve = max(ve, ex[2 * tile(u) + 1]);
+        int least = 1000;
+        most = -1000;
+        for (int u = lane; u < T; u += 64) {
+            most = max(most, ex[WP_HEAD * tile(u) + 1]);
+            least = min(least, ex[WP_HEAD * tile(u) + 3]);
+        }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) ve = max(ve, __shfl_xor(ve, o, 64));
-        ve = __builtin_amdgcn_readfirstlane(ve);
+        for (int o = 32; o > 0; o >>= 1) {
+            most = max(most, __shfl_xor(most, o, 64));
+            least = min(least, __shfl_xor(least, o, 64));
+        }
+        most = __builtin_amdgcn_readfirstlane(most);
+        far = most > __builtin_amdgcn_readfirstlane(least) + WP_FAR;
+        if (far) most = 0;
     }
     const f32x4 zero4 = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 o[RT][DT];
-    float m[RT], mk[RT], l[RT];   // m: reference in log2 units; mk = RW_SCALE - m
+    float m[RT], mk[RT], l[RT];   // m: reference in log2 units (V's exponent with the score); mk = RW_SCALE - m
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         m[rt] = -INFINITY;
@@ -332,7 +387,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     __builtin_amdgcn_s_waitcnt(WAITCNT_VM_LGKM0(0));
     __syncthreads();
     if (u0 + 1 < u1) issue_k(1, u0 + 1);
-    int ek = 0, ev = 0;   // exponents of the tile
+    int ek = 0, ev = 0, wide = 0;   // of the tile
     if (u0 < u1) {
 #pragma unroll
         for (int q = 0; q < KS; q++) {
@@ -342,8 +397,9 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
             score_step(k, q, sc);
         }
         if constexpr (!F16) {
-            ek = ex[2 * tile(u0)];
-            ev = ex[2 * tile(u0) + 1];
+            ek = ex[WP_HEAD * tile(u0)];
+            ev = ex[WP_HEAD * tile(u0) + 1];
+            wide = ex[WP_HEAD * tile(u0) + 2];
         }
     }
     for (int u = u0, st = 0; u < u1; u++, st ^= 1) {
@@ -353,13 +409,19 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
         if (u + 2 < u1) issue_k(st, u + 2);
         if (u + 1 < u1) issue_v(st ^ 1, u + 1);
         const int t = tile(u), p0 = start(t), cnt = limit(t) - p0;
-        float kf = 1.0f, vf = 1.0f;
+        float kf = 1.0f, ve = 0.0f, lk = 1.0f;
+        int le = 0;   // lk = 2^le
+        const int *alone = nullptr;   // (uniform) the positions' own exponents
         if constexpr (!F16) {
             kf = ldexpf(1.0f, ek);
-            vf = ldexpf(1.0f, ev - ve);
+            ve = (float)ev;
+            le = -WP_LEXP - ev;
+            lk = ldexpf(1.0f, le);
+            if (wide) alone = px + (size_t)t * WP_POS + 4 * g;
             const int tn = tile(min(u + 1, u1 - 1));   // (its exponents in time)
-            ek = ex[2 * tn];
-            ev = ex[2 * tn + 1];
+            ek = ex[WP_HEAD * tn];
+            ev = ex[WP_HEAD * tn + 1];
+            wide = ex[WP_HEAD * tn + 2];
         }
         const int top = p0 + TP - 1;
         if (top > first || cnt < TP || (top >= a.sinks && p0 <= last - a.window)) {   // uniform
@@ -374,18 +436,27 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
                     }
         }
         // ---- online softmax: the reference
-        float f[RT], mx[RT];
+        float f[RT], mx[RT], mv[RT], ls[RT], lw[RT];
         bool up = false;
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             // (above 0: a masked score times it stays -inf)
             f[rt] = F16 ? c2[rt] : fmaxf(c2[rt] * kf, 1e-37f);
+            lw[rt] = 0.0f;
+            if (!F16 && alone) {
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        sc[rt][c][i] = fmaf(ldexpf(sc[rt][c][i], alone[16 * c + i]), f[rt], (float)alone[WP_TP + 16 * c + i]);
+                f[rt] = 1.0f;
+            }
             mx[rt] = sc[rt][0][0];
 #pragma unroll
             for (int c = 0; c < CT; c++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) mx[rt] = fmaxf(mx[rt], sc[rt][c][i]);
-            mx[rt] *= f[rt];
+            mx[rt] = fmaf(mx[rt], f[rt], ve);
             up |= mx[rt] > m[rt] + RW_LAZY;
         }
         if (__ballot(up)) {   // (one branch for both row tiles: what follows is one block to schedule)
@@ -403,23 +474,30 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
                 for (int d = 0; d < DT; d++) o[rt][d] *= al;
             }
         }
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) mv[rt] = mk[rt] + ve;
+        if (!F16 && alone) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        lw[rt] += ldexpf(__builtin_amdgcn_exp2f(sc[rt][c][i] + mv[rt]), le - alone[WP_TP + 16 * c + i]);
+            lk = 0.0f;
+        }
         // ---- the weights (P, in two parts) between the next tile's scores, then
         // O^T += V^T P^T.  The order is fixed: a step's operand pieces are read
         // during the one before, and its products run beside its share of the weights'
         // instructions.  (A K stage past the last tile holds an old one: not used.)
         f32x4 sn[RT][CT];
         f16x8 kr[2][2][NP], ph[RT], pl[RT];
-        float ls[RT];
         constexpr int PAIRS = RT * CT * 2;
         auto weights = [&](int x) {   // scores 2x, 2x + 1 of (rt, c, i)
             const int rt = x / (CT * 2), c = x / 2 % CT, i = x % 2 * 2;
-            float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], f[rt], mk[rt]));
-            float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], f[rt], mk[rt]));
+            const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i], f[rt], mv[rt]));
+            const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[rt][c][i + 1], f[rt], mv[rt]));
             ls[rt] += e0 + e1;
-            if constexpr (!F16) {
-                e0 *= vf;
-                e1 *= vf;
-            }
             const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(e0, e1));
             const f16x2 lw = __builtin_bit_cast(
                 f16x2, __builtin_amdgcn_cvt_pkrtz(fmaf((float)hi[0], -1.0f, e0), fmaf((float)hi[1], -1.0f, e1)));
@@ -446,7 +524,11 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) l[rt] += ls[rt];
+        for (int rt = 0; rt < RT; rt++) l[rt] = F16 ? l[rt] + ls[rt] : fmaf(ls[rt], lk, l[rt]) + lw[rt];
+        // (a wave with only products ahead goes first, so that the other wave of its
+        // SIMD has the vector pipe while the matrix pipe is fed: 32 heads, 512 tokens,
+        // fp32 at d_head 128 176 -> 170 us, fp16 128 tokens 41.9 -> 41.4)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < DT; d += 2) {
 #pragma unroll
@@ -464,6 +546,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
             products(kr[(KS + d / 2) & 1], hi, lo, at);
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
 #pragma unroll
         for (int rt = 0; rt < RT; rt++)
 #pragma unroll
@@ -481,7 +564,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
         ls += __shfl_xor(ls, 32, 64);
         const int r = 32 * wid + 16 * rt + col;
         const bool valid = r < nr;
-        const float unit = ldexpf(1.0f, ve), inv = unit / ls;
+        const float unit = F16 ? 1.0f : ldexpf(1.0f, -WP_LEXP), inv = unit / ls;
         const size_t at = ((size_t)kvh * rows + min(r0 + r, rows - 1)) * a.parts + part;
         f32x4 z = zero4;
 #pragma unroll
@@ -493,10 +576,10 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
             else *(f32x4 *)(a.xo + at * DH + 16 * d + 4 * g) = y;
         }
         if (valid && a.parts > 1 && g == 0) {
-            a.xm[at] = m[rt] == -INFINITY ? -INFINITY : -mk[rt];   // of the weights as they are
+            a.xm[at] = m[rt] == -INFINITY ? -INFINITY : (F16 ? 0 : WP_LEXP) - mk[rt];   // of the weights as they are
             a.xl[at] = ls;
         }
-        if (valid && !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f)) odd = odd_row[r] = 1;
+        if (valid && (far || !(z[0] + z[1] + z[2] + z[3] + ls * 0.0f == 0.0f))) odd = odd_row[r] = 1;
     }
     // A masked position is in its tile's products with weight 0, which a V row
     // that is not finite turns into NaN for the rows that do not see it: rows
@@ -526,11 +609,11 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
 #pragma unroll
         for (int d = 0; d < DL; d++) {
             if (a.parts == 1) a.out[qa + d] = s.o[d] / s.l;
-            else a.xo[at * DH + lane * DL + d] = s.o[d];
+            else a.xo[at * DH + lane * DL + d] = ldexpf(s.o[d], -most);
         }
-        if (a.parts > 1 && lane == 0) {
-            a.xm[at] = s.m;
-            a.xl[at] = s.l;
+        if (a.parts > 1 && lane == 0) {   // (V's exponent in m, as in the parts that are not walked again)
+            a.xm[at] = s.m + (float)most;
+            a.xl[at] = ldexpf(s.l, -most);
         }
     }
 }
@@ -542,7 +625,7 @@ size_t wprompt_split_bytes(int n, int n_kv, int d_head, int max_ctx, int window,
 {
     const long seen = std::min((long)max_ctx, (long)std::min(window, max_ctx) + std::min(sinks, max_ctx) + n);
     const size_t tiles = (size_t)n_kv * (ceil_div(seen, WP_TP) + 2);
-    return tiles * (WP_TP * d_head * 8 + 8);
+    return tiles * (WP_TP * d_head * 8 + (WP_HEAD + WP_POS) * sizeof(int));
 }
 
 template <int DH, bool F16>

@@ -268,6 +268,47 @@ def test_prompt_over_caches_of_any_range(ctx, monkeypatch, dh, k_scale, v_scale,
         close(got[i] / v_scale, want / v_scale, tol / v_scale + 2.0**-33 * np.abs(v / v_scale).max(), f"token {i}")
 
 
+@pytest.mark.parametrize("form", ["0", "1"])
+@pytest.mark.parametrize("f16", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dh", [(16, 4, 128), (9, 3, 64), (4, 4, 32)])
+@pytest.mark.parametrize("big,small", [(1e18, 1e-9), (1e30, 1e-30), (6e4, 1e-3), (3e3, 1.0)])
+def test_prompt_large_values_elsewhere(ctx, monkeypatch, heads, kv, dh, f16, form, big, small):
+    """Finite but large K and V rows, next to ordinary ones and next to rows
+    of small values: tokens that do not see them, or give them no weight, come
+    out as without them.  Every query has 3 in its first dimension, so `low`
+    scores -3 big / sqrt(d_head), a weight of exp(-500) and less, 0.  Absolute
+    term: a V row is held to 2^-33 of its largest."""
+    prompt_form(monkeypatch, form)
+    n, pos0, max_ctx, window, sinks = 90, 40, 160, 30, 2
+    rng = np.random.default_rng(11)
+    q = rng.standard_normal((n, heads, dh)).astype(np.float32)
+    q[..., 0] = 3
+    k, v = (rand_cache(rng, (kv, max_ctx, dh), f16) for _ in range(2))
+    if f16:
+        big, small = min(big, 6e4), max(small, 1e-3)
+    low, seen_big = [45, 88, 110], [0, 60, 99, 129]
+    v[:, 20:28] *= v.dtype.type(small)
+    v[:, 70:75] *= v.dtype.type(small)
+    k[:, 84:86] *= k.dtype.type(small)
+    k[:, 112], v[:, 114] = 0, 0
+    k[:, low] = 0
+    k[:, low, 0] = -big
+    v[:, low] = np.sign(v[:, low]) * v.dtype.type(big)
+    v[:, seen_big[1:]] = np.sign(v[:, seen_big[1:]]) * v.dtype.type(big)
+    got = prompt_call(ctx, q, ctx.upload(k), ctx.upload(v), pos0, heads, kv, dh, max_ctx, f16, window, sinks)
+    k64, v64 = k.astype(np.float64), v.astype(np.float64)
+    for i in range(n):
+        seen = window_seen(pos0 + i + 1, max_ctx, window, sinks)
+        seen[low] = False
+        want, tol = reference(q[i].astype(np.float64), k64, v64, seen)
+        tops = np.repeat(np.abs(v64).max(2, keepdims=True), dh, 2)
+        for h in range(heads):
+            s = k64[h * kv // heads][seen] @ q[i, h].astype(np.float64) / np.sqrt(dh)
+            w = np.exp(s - s.max())
+            tol[h] += 2.0**-33 * (w / w.sum()) @ tops[h * kv // heads][seen]
+        close(got[i], want, tol, f"token {i}")
+
+
 def test_prompt_tokens_equal_single_tokens(ctx):
     """A prompt's rows and the same tokens decoded one by one, as sessions
     over one cache."""
