@@ -19,23 +19,26 @@
 //     query rows, so lane (col, g) holds positions 4g .. 4g+3 of row `col` (of each
 //     16);
 //   * O^T += V^T P^T: the scores' layout is the B operand's as it is (k index
-//     of lane group g = positions 4g .. 4g+3, and 16 more of the tile's second
-//     16, over fp16), and a lane's A operand for output tile e is dimension VD col + e of
-//     those positions, VD = d_head / 16: a lane loads VD neighbouring dimensions
-//     of its positions' V rows, 16 lanes a whole row, and for fp16 pairs of rows
-//     are interleaved with one v_perm_b32 per two values;
+//     of lane group g = positions 4g .. 4g+3, and over fp16 those of the tile's
+//     second 16), and a lane's A operand for output tile e is dimension
+//     VD col + e of those positions, VD = d_head / 16: a lane loads VD neighbouring
+//     dimensions of its positions' V rows, 16 lanes a whole row, and for fp16
+//     pairs of rows are interleaved with one v_perm_b32 per two values;
 //   * online softmax whose reference moves only when a score exceeds it by more
 //     than RW_LAZY (log2 units; a wave vote), so most tiles need no cross-lane
 //     step; weights are 2^(t c2 + mk), c2 = log2(e) / sqrt(d_head).
 // fp16 caches: 16x16x32 f16 products, exact, with fp32 sums.  The query is
 // scaled by a power of two per row into [2^9, 2^10) and split into two f16 parts
-// (22 bits, 2^-33 of the row's largest below) whose products share a sum; a weight, scaled by 2^RW_SCALE, into two f16 parts whose products
-// share an accumulator (22 bits of a weight down to 2^-16 of the largest, an
-// absolute 2^-36 of it below).  fp32 caches: 16x16x4 f32 products throughout.
+// (22 bits, 2^-33 of the row's largest below) whose products share a sum; a
+// weight, scaled by 2^RW_SCALE, into two f16 parts whose products share an
+// accumulator (22 bits of a weight down to 2^-16 of the largest, an absolute
+// 2^-36 of it below).  fp32 caches: 16x16x4 f32 products throughout; a few rows
+// by themselves have a walk of their own (few_walk).
 #pragma once
 #include "common.h"
 
 #include <algorithm>
+#include <utility>
 
 template <typename KT> constexpr int rw_tp() { return sizeof(KT) == 2 ? 32 : 16; }   // positions per tile
 constexpr int RW_PAD = 2;            // tiles that stand for the start of an item's piece
@@ -76,6 +79,18 @@ struct RowsLine {
     {
         *p0 = u < ns ? u * TP : lo + (u - ns) * TP;
         *cnt = min(TP, (u < ns ? s : hi) - *p0);
+    }
+    // in scalar registers: what follows from them is too, and branches on it are
+    // scalar ones (the lines and ranges of a wave are uniform, which the compiler
+    // cannot see through the search of a piece)
+    __device__ __forceinline__ RowsLine uniform() const
+    {
+        RowsLine x;
+        x.s = __builtin_amdgcn_readfirstlane(s);
+        x.lo = __builtin_amdgcn_readfirstlane(lo);
+        x.hi = __builtin_amdgcn_readfirstlane(hi);
+        x.ns = __builtin_amdgcn_readfirstlane(ns);
+        return x;
     }
 };
 
@@ -309,9 +324,12 @@ struct RowsSeen {
 // different positions (seen).
 template <int DH, typename KT, int RT, bool MASKED>
 __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb, const KT *vb,
-                                          const RowsLine<rw_tp<KT>()> &line, int u, int u1, int step, const RowsSeen *seen)
+                                          const RowsLine<rw_tp<KT>()> &line0, int u, int u1, int step, const RowsSeen *seen)
 {
 #pragma clang fp contract(off)
+    const auto line = line0.uniform();
+    u = __builtin_amdgcn_readfirstlane(u);
+    u1 = __builtin_amdgcn_readfirstlane(u1);
     typedef RowsWave<DH, KT, RT> W;
     constexpr bool F16 = W::F16;
     constexpr int VD = W::VD, KS = W::KS, ES = sizeof(KT), TP = rw_tp<KT>(), C = TP / 16, VR = TP / 4;
@@ -568,6 +586,244 @@ __device__ __forceinline__ void rows_store(float *p, const float (&x)[N])
 #pragma unroll
         for (int e = 0; e < N; e++) p[e] = x[e];
     }
+}
+
+// ---- few rows over fp32 ----------------------------------------------------------
+// At most four query rows of a kv head (its group, for single tokens) over an
+// fp32 cache at d_head 64 and 128.  Of the 16 columns of a 16x16x4 f32 product
+// they would use four; 4x4x1 f32 products, 16 blocks an instruction, run at the
+// same rate and waste none.  Tiles of 32 positions:
+//   * a cached row is GL = d_head / 4 lanes of 16 bytes, an instruction loads NQ =
+//     64 / GL whole rows: load n of a tile rows NQ n + q, q = lane / GL;
+//   * scores: the quads' lanes hold dimensions, the products want positions: four
+//     loads' registers are transposed within the quads (two DPP exchanges), lane t
+//     then holds position 4i + t of the loads (A) against the four rows (B) over
+//     16 dimensions of its block.  The sums over the blocks of a row are
+//     reduce-scattered (lane swaps of 16, DPP for 8 and 4): lane 4b + h ends
+//     with two positions of row h, those of V loads 2 (b % (GL / 4)) + 0 and 1;
+//   * that is the A operand of the second product, whose blocks of a V row's
+//     lanes share one position: the broadcast takes it from one block of each
+//     group of GL / 4.
+// Bound by the cache's bytes on their way into the CUs.  16 sessions of 15/5 heads
+// of 64, windows of 601: 9.95 us by 16x16x4 products, 8.0 by these; 100 sessions
+// 21.1, 19.8; 64 of windows of 2000 66, 62; 48 sessions' own positions behind a
+// prefix (d_head 128) 21.7, 18.9 in the kernel; one session's window of 128 alike.
+constexpr int FEW_ROWS = 4, FEW_TP = 32;
+constexpr bool few_takes(int d_head, int group, int kv_f16)
+{
+    return !kv_f16 && group <= FEW_ROWS && (d_head == 64 || d_head == 128);
+}
+
+template <int DH, int NW>
+struct FewMeet {
+    __attribute__((aligned(16))) float o[NW][FEW_ROWS][DH];
+    float m[NW][FEW_ROWS], l[NW][FEW_ROWS];
+};
+
+template <int DH>
+struct RowsFew {
+    static constexpr int GL = DH / 4, NQ = 64 / GL, NV = FEW_TP / NQ;
+    f32x4 q[4];     // q[t][e]: dimension 16 (b % (GL / 4)) + 4t + e of row h
+    f32x4 o[4];     // o[e][h]: dimension 4 (lane % GL) + e of row h, the positions of group lane / GL
+    float m, mk, l; // of row h; l: this lane's positions only
+    template <typename Q>
+    __device__ __forceinline__ void load(Q at)
+    {
+        const int lane = threadIdx.x & 63;
+        const float *p = at(lane & 3) + 16 * (lane % GL / 4);
+#pragma unroll
+        for (int t = 0; t < 4; t++) q[t] = ldg((const f32x4 *)(p + 4 * t));
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        m = -INFINITY;
+        mk = RW_SCALE;
+        l = 0.0f;
+    }
+    // V rows n of every group, the weights of block n / 2 of each
+    template <int... N>
+    __device__ __forceinline__ void add(const f32x4 (&v)[NV], const float (&p)[2], std::integer_sequence<int, N...>)
+    {
+        (add_one<N>(v[N], p[N & 1]), ...);
+    }
+    template <int N>
+    __device__ __forceinline__ void add_one(f32x4 v, float p)
+    {
+        // (one value of four registers up to here: the compiler gave a lane of it
+        // away to the weights' arithmetic, before its product)
+        asm volatile("" : "+v"(v));
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = __builtin_amdgcn_mfma_f32_4x4x1f32(p, v[e], o[e], GL == 16 ? 2 : 3, N >> 1, 0);
+    }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float few_dpp(float x)
+{
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+
+// Two registers' transposition with the lane that DPP control CTRL names: the
+// lower one's (on false) second against the upper one's first.
+template <int CTRL>
+__device__ __forceinline__ void few_exchange(bool on, float a, float b, float &x, float &y)
+{
+    const float fa = few_dpp<CTRL>(a), fb = few_dpp<CTRL>(b);   // (by every lane: not in the selection)
+    x = on ? fb : a;
+    y = on ? b : fa;
+}
+
+// As rows_walk: tiles u, u + step, .. below u1.
+template <int DH>
+__device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const float *vb, const RowsLine<FEW_TP> &line0, int u,
+                                         int u1, int step)
+{
+#pragma clang fp contract(off)
+    const auto line = line0.uniform();
+    u = __builtin_amdgcn_readfirstlane(u);
+    u1 = __builtin_amdgcn_readfirstlane(u1);
+    typedef RowsFew<DH> W;
+    constexpr int TP = FEW_TP, GL = W::GL, NQ = W::NQ, NV = W::NV, NJ = NV / 4;
+    const int lane = threadIdx.x & 63, b = lane >> 2, q = lane / GL;
+    const float c2 = 1.44269504088896341f / sqrtf((float)DH);
+    f32x4 kr[NV], vr[NV];
+    auto load = [&](const float *from, int t, f32x4 (&to)[NV]) {
+        int p0, cnt;
+        line.tile(t, &p0, &cnt);
+        const char *base = (const char *)uniform_ptr(from + (size_t)p0 * DH);
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+            to[n] = ldg((const f32x4 *)(base + ((unsigned)min(NQ * n + q, cnt - 1) * (DH * 4) + 16 * (lane % GL))));
+    };
+    if (u >= u1) return;
+    load(kb, u, kr);
+    load(vb, u, vr);
+    for (;;) {
+        const bool more = u + step < u1;
+        int p0, cnt;
+        line.tile(u, &p0, &cnt);
+        f32x4 s[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; j++) s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const bool l1 = lane & 1, l2 = lane & 2;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            float z[NJ][4];
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const float r0 = kr[4 * j][e], r1 = kr[4 * j + 1][e], r2 = kr[4 * j + 2][e], r3 = kr[4 * j + 3][e];
+                float y0, y1, y2, y3;
+                few_exchange<0xb1>(l1, r0, r1, y0, y1);   // quad_perm: the lane 1 away
+                few_exchange<0xb1>(l1, r2, r3, y2, y3);
+                few_exchange<0x4e>(l2, y0, y2, z[j][0], z[j][2]);   // (2 away)
+                few_exchange<0x4e>(l2, y1, y3, z[j][1], z[j][3]);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) s[j] = __builtin_amdgcn_mfma_f32_4x4x1f32(z[j][t], w.q[t][e], s[j], 0, 0, 0);
+        }
+        if (more) load(kb, u + step, kr);
+        // ---- reduce-scatter: x[4j + i] is row NQ (4j + i) + q of the tile
+        float x[NV], p[2];
+#pragma unroll
+        for (int i = 0; i < NV; i++) x[i] = s[i / 4][i % 4];
+        if constexpr (GL == 32) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x[i]), __float_as_uint(x[i + 8]), false, false);
+                x[i] = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool on = lane & 8;
+            x[i] = (on ? x[i + 4] : x[i]) + few_dpp<0x128>(on ? x[i] : x[i + 4]);   // row_ror 8: the lane 8 away
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const bool on = lane & 4;   // (mirrored halves of a row, mirrored quads: the lane 4 away)
+            p[i] = (on ? x[i + 2] : x[i]) + few_dpp<0x1b>(few_dpp<0x141>(on ? x[i] : x[i + 2]));
+        }
+        // ---- the run's end: V rows past it 0, not a copy of its last (0 weight times infinity)
+        if (cnt < TP) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                if (NQ * (2 * (b % (GL / 4)) + i) + q >= cnt) p[i] = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < NV; n++)
+                if (NQ * n + q >= cnt) vr[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        // ---- online softmax
+        float mx = fmaxf(p[0], p[1]);
+        if (__ballot((mx - w.m) * c2 > RW_LAZY)) {
+#pragma unroll
+            for (int o = 4; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+            const float mn = fmaxf(w.m, mx), mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn * c2;
+            const float al = w.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - w.mk);
+            w.m = mn;
+            w.mk = mkn;
+            w.l *= al;
+#pragma unroll
+            for (int h = 0; h < FEW_ROWS; h++) {
+                const float f = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(al), h));
+#pragma unroll
+                for (int e = 0; e < 4; e++) w.o[e][h] *= f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], c2, w.mk));
+            w.l += p[i];
+        }
+        w.add(vr, p, std::make_integer_sequence<int, NV>());
+        if (!more) return;
+        u += step;
+        load(vb, u, vr);
+    }
+}
+
+// As rows_finish, put(r, m, l, d, x) for rows below FEW_ROWS.
+template <int DH, int NW, typename P>
+__device__ __forceinline__ void few_finish(RowsFew<DH> &w, FewMeet<DH, NW> &meet, P put)
+{
+#pragma clang fp contract(off)
+    constexpr int GL = RowsFew<DH>::GL;
+    const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+    float l = w.l;
+#pragma unroll
+    for (int o = 4; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+#pragma unroll
+    for (int o = GL; o < 64; o <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int h = 0; h < FEW_ROWS; h++) w.o[e][h] += __shfl_xor(w.o[e][h], o, 64);
+    if (lane < FEW_ROWS) {
+        meet.m[wid][lane] = w.m == -INFINITY ? -INFINITY : -w.mk;
+        meet.l[wid][lane] = l;
+    }
+    if (lane < GL) {
+#pragma unroll
+        for (int h = 0; h < FEW_ROWS; h++)
+            *(f32x4 *)&meet.o[wid][h][4 * lane] = f32x4{w.o[0][h], w.o[1][h], w.o[2][h], w.o[3][h]};
+    }
+    __syncthreads();
+    if (tid >= FEW_ROWS * GL) return;
+    const int r = tid / GL, d = 4 * (tid % GL);
+    float mx = meet.m[0][r];
+#pragma unroll
+    for (int k = 1; k < NW; k++) mx = fmaxf(mx, meet.m[k][r]);
+    const float ref = mx == -INFINITY ? 0.0f : mx;
+    float lt = 0.0f, x[4] = {};
+#pragma unroll
+    for (int k = 0; k < NW; k++) {
+        const float f = __builtin_amdgcn_exp2f(meet.m[k][r] - ref);
+        lt += meet.l[k][r] * f;
+        const f32x4 y = *(const f32x4 *)&meet.o[k][r][d];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += y[e] * f;
+    }
+    put(r, mx, lt, d, x);
 }
 
 // ---- one row on one wave ---------------------------------------------------------

@@ -51,24 +51,26 @@ __device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH, SH
     });
 }
 
-template <int DH, typename KT>
-__device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH, SH_NW> &meet, unsigned wg)
+template <int DH, typename KT, bool FEW, typename M>
+__device__ __forceinline__ void shared_own(const RowsArgs &a, M &meet, unsigned wg)
 {
 #pragma clang fp contract(off)
     const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
     const int slot = wg / (a.n_kv * blocks), hb = wg % (a.n_kv * blocks), kvh = hb / blocks, r0 = hb % blocks * 16;
     const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    constexpr int TP = rw_tp<KT>();
+    constexpr int TP = FEW ? FEW_TP : rw_tp<KT>();
     const RowsPiece p = rows_piece<TP>(a, slot);
     if (p.item < 0 || p.L <= 0) return;
     const RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
     const size_t row0 = (size_t)p.item * a.n_heads + (size_t)kvh * G;
-    RowsWave<DH, KT, 1> w;
+    typename std::conditional<FEW, RowsFew<DH>, RowsWave<DH, KT, 1>>::type w;
     w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     const size_t base = (size_t)p.slot * a.slot_stride + (size_t)kvh * a.max_ctx * DH;
-    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, p.u0 + wid, p.u1, SH_NW, nullptr);
+    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
+    if constexpr (FEW) few_walk<DH>(w, k, v, line, p.u0 + wid, p.u1, SH_NW);
+    else rows_walk<DH, KT, 1, false>(w, k, v, line, p.u0 + wid, p.u1, SH_NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
-    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+    auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
         rows_store(a.po + (part + r) * DH + d, x);
@@ -76,16 +78,22 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, RowsMeet<DH, SH_NW
             a.pm[part + r] = m;
             a.pl[part + r] = l;
         }
-    });
+    };
+    if constexpr (FEW) few_finish(w, meet, put);
+    else rows_finish(w, meet, put);
 }
 
-template <int DH, typename KT, int RT>
+template <int DH, typename KT, int RT, bool FEW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_shared(RowsArgs a)
 {
-    __shared__ RowsMeet<DH, SH_NW> meet;
+    __shared__ union {
+        RowsMeet<DH, SH_NW> rows;
+        FewMeet<DH, SH_NW> few;
+    } meet;
     const unsigned pre = shared_prefix_wgs(a, RT);
-    if (blockIdx.x < pre) shared_prefix<DH, KT, RT>(a, meet, blockIdx.x);
-    else shared_own<DH, KT>(a, meet, blockIdx.x - pre);
+    if (blockIdx.x < pre) shared_prefix<DH, KT, RT>(a, meet.rows, blockIdx.x);
+    else if constexpr (FEW) shared_own<DH, KT, true>(a, meet.few, blockIdx.x - pre);
+    else shared_own<DH, KT, false>(a, meet.rows, blockIdx.x - pre);
 }
 
 template <int DH, int TP>
@@ -152,14 +160,17 @@ int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
     const int G = a.n_heads / a.n_kv, rt = shared_rt(a.n, G, a.d_head, a.kv_f16);
     a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt, a.kv_f16));
     const dim3 grid(shared_prefix_wgs(a, rt) + (unsigned)(a.n_kv * ceil_div(G, 16)) * (a.bal + a.n)), block(256);
-#define SHA(DH)                                                                                          \
-    if (!a.kv_f16) hipLaunchKernelGGL((k_shared<DH, float, 1>), grid, block, 0, s, a);                   \
-    else if (DH == 256 || rt == 1) hipLaunchKernelGGL((k_shared<DH, _Float16, 1>), grid, block, 0, s, a); \
-    else hipLaunchKernelGGL((k_shared<DH, _Float16, DH == 256 ? 1 : 2>), grid, block, 0, s, a);
+    const bool few = few_takes(a.d_head, G, a.kv_f16);
+#define SHA(DH)                                                                                                  \
+    if constexpr (few_takes(DH, 1, 0))                                                                           \
+        if (few) hipLaunchKernelGGL((k_shared<DH, float, 1, true>), grid, block, 0, s, a);                       \
+    if (!a.kv_f16 && !few) hipLaunchKernelGGL((k_shared<DH, float, 1, false>), grid, block, 0, s, a);            \
+    if (a.kv_f16 && (DH == 256 || rt == 1)) hipLaunchKernelGGL((k_shared<DH, _Float16, 1, false>), grid, block, 0, s, a); \
+    if (a.kv_f16 && rt == 2) hipLaunchKernelGGL((k_shared<DH, _Float16, DH == 256 ? 1 : 2, false>), grid, block, 0, s, a);
     RW_BY_D_HEAD(a.d_head, SHA)
 #undef SHA
 #define MERGE(DH)                                                                                     \
-    if (a.kv_f16) hipLaunchKernelGGL((k_shared_merge<DH, 32>), dim3(a.n_heads, a.n), block, 0, s, a); \
+    if (a.kv_f16 || few) hipLaunchKernelGGL((k_shared_merge<DH, 32>), dim3(a.n_heads, a.n), block, 0, s, a); \
     else hipLaunchKernelGGL((k_shared_merge<DH, 16>), dim3(a.n_heads, a.n), block, 0, s, a);
     RW_BY_D_HEAD(a.d_head, MERGE)
 #undef MERGE

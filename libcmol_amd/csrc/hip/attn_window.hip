@@ -8,12 +8,12 @@
 
 // Work-group of NW waves (16 query heads of a kv head, slot): the piece of that
 // slot, or item `slot` whole where there are no balanced ranges.
-template <int DH, typename KT, int NW>
+template <int DH, typename KT, int NW, bool FEW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window(RowsArgs a)
 {
 #pragma clang fp contract(off)
-    constexpr int TP = rw_tp<KT>();
-    __shared__ RowsMeet<DH, NW> meet;
+    constexpr int TP = FEW ? FEW_TP : rw_tp<KT>();
+    __shared__ typename std::conditional<FEW, FewMeet<DH, NW>, RowsMeet<DH, NW>>::type meet;
     const int G = a.n_heads / a.n_kv, blocks = (G + 15) / 16;
     const int kvh = blockIdx.x / blocks, r0 = (blockIdx.x % blocks) * 16, slot = blockIdx.y;
     const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -21,12 +21,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 2
     if (p.item < 0) return;
     const RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
     const size_t row0 = (size_t)p.item * a.n_heads + (size_t)kvh * G;
-    RowsWave<DH, KT, 1> w;
+    typename std::conditional<FEW, RowsFew<DH>, RowsWave<DH, KT, 1>>::type w;
     w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     const size_t base = (p.L > 0 ? (size_t)p.slot * a.slot_stride : 0) + (size_t)kvh * a.max_ctx * DH;
-    rows_walk<DH, KT, 1, false>(w, (const KT *)a.k + base, (const KT *)a.v + base, line, p.u0 + wid, p.u1, NW, nullptr);
+    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
+    if constexpr (FEW) few_walk<DH>(w, k, v, line, p.u0 + wid, p.u1, NW);
+    else rows_walk<DH, KT, 1, false>(w, k, v, line, p.u0 + wid, p.u1, NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
-    rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
+    auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
         if (p.whole) {
@@ -40,7 +42,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 2
                 a.pl[part + r] = l;
             }
         }
-    });
+    };
+    if constexpr (FEW) few_finish(w, meet, put);
+    else rows_finish(w, meet, put);
 }
 
 // One work-group per (query head, item): the item's pieces.
@@ -273,18 +277,24 @@ int launch_attn_window(const RowsArgs &a, hipStream_t s)
     // eight waves for items that have more than one round of tiles for four
     // (d_head 256: four, for their registers)
     const bool wide = !a.bal && a.d_head < 256 && span_tiles(a.max_ctx, a.window, a.sinks) > 4;
-#define LAUNCH(DH, KT, NW) hipLaunchKernelGGL((k_window<DH, KT, NW>), grid, dim3(NW * 64), 0, s, a)
-#define WIN(DH)                                                               \
-    if constexpr (DH < 256) {                                                 \
-        if (wide) { if (a.kv_f16) LAUNCH(DH, _Float16, 8); else LAUNCH(DH, float, 8); }   \
-    }                                                                         \
-    if (!wide) { if (a.kv_f16) LAUNCH(DH, _Float16, 4); else LAUNCH(DH, float, 4); }
+    const bool few = few_takes(a.d_head, a.n_heads / a.n_kv, a.kv_f16);
+#define LAUNCH(DH, KT, NW, FEW) hipLaunchKernelGGL((k_window<DH, KT, NW, FEW>), grid, dim3(NW * 64), 0, s, a)
+#define WIN_NW(DH, NW)                                        \
+    if constexpr (few_takes(DH, 1, 0))                        \
+        if (few) LAUNCH(DH, float, NW, true);                 \
+    if (a.kv_f16) LAUNCH(DH, _Float16, NW, false);            \
+    else if (!few) LAUNCH(DH, float, NW, false);
+#define WIN(DH)                                               \
+    if constexpr (DH < 256)                                   \
+        if (wide) { WIN_NW(DH, 8) }                           \
+    if (!wide) { WIN_NW(DH, 4) }
     RW_BY_D_HEAD(a.d_head, WIN)
 #undef WIN
+#undef WIN_NW
 #undef LAUNCH
     if (a.bal) {
 #define MERGE(DH)                                                                                              \
-    if (a.kv_f16) hipLaunchKernelGGL((k_window_merge<DH, 32>), dim3(a.n_heads, a.n), dim3(256), 0, s, a);      \
+    if (a.kv_f16 || few) hipLaunchKernelGGL((k_window_merge<DH, 32>), dim3(a.n_heads, a.n), dim3(256), 0, s, a);      \
     else hipLaunchKernelGGL((k_window_merge<DH, 16>), dim3(a.n_heads, a.n), dim3(256), 0, s, a);
         RW_BY_D_HEAD(a.d_head, MERGE)
 #undef MERGE
