@@ -35,7 +35,7 @@
 // 2^-36 of it below).  fp32 caches: 16x16x4 f32 products throughout; a few rows
 // by themselves have a walk of their own (few_walk).
 #pragma once
-#include "common.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <utility>
@@ -127,22 +127,6 @@ __device__ __forceinline__ unsigned rows_tiles(const RowsArgs &a, int L)
 // piece, in slot w + i (unique: pieces are in line order), so an item's pieces
 // are consecutive slots and every work-group of `bal + n` finds its own piece,
 // if any, from the lengths alone.
-__device__ __forceinline__ unsigned wave_sum_u(unsigned v)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-__device__ __forceinline__ unsigned wave_scan_u(unsigned v)   // inclusive
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const unsigned t = __shfl_up(v, o, 64);
-        if (lane >= o) v += t;
-    }
-    return v;
-}
 constexpr unsigned RW_RMIN = 4;   // tiles per range at least: one per wave
 
 // A lane's item among the first 64, and the range length (every wave works
@@ -284,8 +268,7 @@ struct RowsWave {
                     if (DH < 32 && g >= 2) x[rt][i] = 0.0f;   // (d_head 16: half a k-step)
                     top = fmaxf(top, fabsf(x[rt][i]));
                 }
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                top = lanes_max<32>(lanes_max<16>(top));
                 // the largest into [2^9, 2^10), so that the low parts are normal
                 // numbers too (below 2^-100 less, so that c2 stays above 0); a row
                 // of zeros, infinities or NaN as it is
@@ -456,8 +439,7 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
         if (__ballot(up)) {
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 16, 64));
-                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 32, 64));
+                mx[rt] = lanes_max<32>(lanes_max<16>(mx[rt]));
                 const float mn = fmaxf(w.m[rt], mx[rt]);
                 const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn * w.c2[rt];
                 const float al = w.m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - w.mk[rt]);
@@ -540,9 +522,7 @@ __device__ __forceinline__ void rows_finish(RowsWave<DH, KT, RT> &w, RowsMeet<DH
     const int r = tid / TPR, a = tid % TPR;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        float l = w.l[rt];
-        l += __shfl_xor(l, 16, 64);
-        l += __shfl_xor(l, 32, 64);
+        const float l = lanes_add<32>(lanes_add<16>(w.l[rt]));
         // a lane's dimensions VD (4g + i) .. +VD-1 of round c: those in [c DC, c DC + DC)
 #pragma unroll
         for (int c = 0; c < DH / DC; c++) {
@@ -656,18 +636,12 @@ struct RowsFew {
     }
 };
 
-template <int CTRL>
-__device__ __forceinline__ float few_dpp(float x)
-{
-    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
-}
-
-// Two registers' transposition with the lane that DPP control CTRL names: the
-// lower one's (on false) second against the upper one's first.
-template <int CTRL>
+// Two registers' transposition with the lane O away: the lower one's (on
+// false) second against the upper one's first.
+template <int O>
 __device__ __forceinline__ void few_exchange(bool on, float a, float b, float &x, float &y)
 {
-    const float fa = few_dpp<CTRL>(a), fb = few_dpp<CTRL>(b);   // (by every lane: not in the selection)
+    const float fa = lane_xor<O>(a), fb = lane_xor<O>(b);
     x = on ? fb : a;
     y = on ? b : fa;
 }
@@ -712,10 +686,10 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
             for (int j = 0; j < NJ; j++) {
                 const float r0 = kr[4 * j][e], r1 = kr[4 * j + 1][e], r2 = kr[4 * j + 2][e], r3 = kr[4 * j + 3][e];
                 float y0, y1, y2, y3;
-                few_exchange<0xb1>(l1, r0, r1, y0, y1);   // quad_perm: the lane 1 away
-                few_exchange<0xb1>(l1, r2, r3, y2, y3);
-                few_exchange<0x4e>(l2, y0, y2, z[j][0], z[j][2]);   // (2 away)
-                few_exchange<0x4e>(l2, y1, y3, z[j][1], z[j][3]);
+                few_exchange<1>(l1, r0, r1, y0, y1);
+                few_exchange<1>(l1, r2, r3, y2, y3);
+                few_exchange<2>(l2, y0, y2, z[j][0], z[j][2]);
+                few_exchange<2>(l2, y1, y3, z[j][1], z[j][3]);
             }
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -737,12 +711,12 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const bool on = lane & 8;
-            x[i] = (on ? x[i + 4] : x[i]) + few_dpp<0x128>(on ? x[i] : x[i + 4]);   // row_ror 8: the lane 8 away
+            x[i] = (on ? x[i + 4] : x[i]) + lane_xor<8>(on ? x[i] : x[i + 4]);
         }
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const bool on = lane & 4;   // (mirrored halves of a row, mirrored quads: the lane 4 away)
-            p[i] = (on ? x[i + 2] : x[i]) + few_dpp<0x1b>(few_dpp<0x141>(on ? x[i] : x[i + 2]));
+            const bool on = lane & 4;
+            p[i] = (on ? x[i + 2] : x[i]) + lane_xor<4>(on ? x[i] : x[i + 2]);
         }
         // ---- the run's end: V rows past it 0, not a copy of its last (0 weight times infinity)
         if (cnt < TP) {
@@ -756,8 +730,7 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
         // ---- online softmax
         float mx = fmaxf(p[0], p[1]);
         if (__ballot((mx - w.m) * c2 > RW_LAZY)) {
-#pragma unroll
-            for (int o = 4; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+            mx = lanes_max<32>(lanes_max<16>(lanes_max<8>(lanes_max<4>(mx))));
             const float mn = fmaxf(w.m, mx), mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn * c2;
             const float al = w.m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - w.mk);
             w.m = mn;
@@ -789,15 +762,11 @@ __device__ __forceinline__ void few_finish(RowsFew<DH> &w, FewMeet<DH, NW> &meet
 #pragma clang fp contract(off)
     constexpr int GL = RowsFew<DH>::GL;
     const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-    float l = w.l;
+    const float l = lanes_add<32>(lanes_add<16>(lanes_add<8>(lanes_add<4>(w.l))));
 #pragma unroll
-    for (int o = 4; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+    for (int e = 0; e < 4; e++)
 #pragma unroll
-    for (int o = GL; o < 64; o <<= 1)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int h = 0; h < FEW_ROWS; h++) w.o[e][h] += __shfl_xor(w.o[e][h], o, 64);
+        for (int h = 0; h < FEW_ROWS; h++) w.o[e][h] = lanes_add<32>(GL == 16 ? lanes_add<16>(w.o[e][h]) : w.o[e][h]);
     if (lane < FEW_ROWS) {
         meet.m[wid][lane] = w.m == -INFINITY ? -INFINITY : -w.mk;
         meet.l[wid][lane] = l;

@@ -282,8 +282,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
                 top = fmaxf(top, fabsf(x[s][e]));
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = lanes_max<32>(lanes_max<16>(top));
         const int e0 = top > 0.0f && top < INFINITY ? max(ilogbf(top), -100) - 9 : 0;
         c2[rt] = ldexpf(1.44269504088896341f / sqrtf((float)DH), e0);
 #pragma unroll
@@ -462,8 +461,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
         if (__ballot(up)) {   // (one branch for both row tiles: what follows is one block to schedule)
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
-                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 16, 64));
-                mx[rt] = fmaxf(mx[rt], __shfl_xor(mx[rt], 32, 64));
+                mx[rt] = lanes_max<32>(lanes_max<16>(mx[rt]));
                 const float mn = fmaxf(m[rt], mx[rt]);
                 const float mkn = mn == -INFINITY ? RW_SCALE : RW_SCALE - mn;
                 const float al = m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mkn - mk[rt]);
@@ -559,9 +557,7 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
     __syncthreads();
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        float ls = l[rt];
-        ls += __shfl_xor(ls, 16, 64);
-        ls += __shfl_xor(ls, 32, 64);
+        const float ls = lanes_add<32>(lanes_add<16>(l[rt]));
         const int r = 32 * wid + 16 * rt + col;
         const bool valid = r < nr;
         const float unit = F16 ? 1.0f : ldexpf(1.0f, -WP_LEXP), inv = unit / ls;

@@ -19,16 +19,19 @@
 // every work-group reads the row's history, so where the rows alone give each CU
 // one slabs are large (SLAB 8192 on 1024 threads), else small (2048 on 256).
 #include "logits.h"
+#include "lanes.h"
 
+// The largest key of a wave: the largest upper half, then the largest lower one
+// among the lanes that have it.
 __device__ inline unsigned long long key_max(unsigned long long k)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t hi = __shfl_xor((uint32_t)(k >> 32), o, 64), lo = __shfl_xor((uint32_t)k, o, 64);
-        const unsigned long long x = ((unsigned long long)hi << 32) | lo;
-        k = x > k ? x : k;
-    }
-    return k;
+    auto most = [](uint32_t x) {
+        auto f = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+        return lanes_pair<32>(
+            lanes_pair<16>(lanes_pair<8>(lanes_pair<4>(lanes_pair<2>(lanes_pair<1>(x, f), f), f), f), f), f);
+    };
+    const uint32_t hi = most((uint32_t)(k >> 32)), lo = most((uint32_t)(k >> 32) == hi ? (uint32_t)k : 0);
+    return ((unsigned long long)hi << 32) | lo;
 }
 
 // x / rep rounded, y = 1 / rep rounded, for 2^-60 <= x <= 2^100 and rep <= 2^30
