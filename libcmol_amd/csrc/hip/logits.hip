@@ -34,21 +34,25 @@ __device__ inline unsigned long long key_max(unsigned long long k)
     return ((unsigned long long)hi << 32) | lo;
 }
 
-// x / rep rounded, y = 1 / rep rounded, for 2^-60 <= x <= 2^100 and rep <= 2^30
-// (every step stays among the normal numbers): the quotient by y is within 1.5
-// ulp, one correction brings it within one, and with the remainder then exact a
-// second one rounds it as the division does (Markstein).
-__device__ inline float divide_step(float x, float rep, float y)
+// 1 / rep in two parts, the first of them rounded.
+struct Reciprocal {
+    float hi, lo;
+    __device__ explicit Reciprocal(float rep) : hi(1.0f / rep), lo(fmaf(-rep, hi, 1.0f) * hi) {}
+};
+// x / rep rounded, for 2^-60 <= x <= 2^100 and rep <= 2^30 (every step stays among
+// the normal numbers): the product with both parts is off by its last rounding
+// and 2^-23 ulp, so within one ulp, and then the remainder is exact and one
+// correction by the rounded reciprocal rounds it as the division does (Markstein).
+__device__ inline float divide_step(float x, float rep, Reciprocal y)
 {
-    float q = x * y;
-    q = fmaf(fmaf(-rep, q, x), y, q);
-    return fmaf(fmaf(-rep, q, x), y, q);
+    const float q = fmaf(x, y.hi, x * y.lo);
+    return fmaf(fmaf(-rep, q, x), y.hi, q);
 }
 
 // The repeat penalty of c occurrences.  Eight steps at a time where there are
 // as many: a word that fills its history is a chain of hundreds of dependent
 // steps on one lane (32 rows, 211 occurrences at most: 11 us with a check a step).
-__device__ inline float repeat_penalty(float x, int c, float rep, float y)
+__device__ inline float repeat_penalty(float x, int c, float rep, Reciprocal y)
 {
 #pragma clang fp contract(off)
     if (x > 0.0f) {
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(NT) void k_logits(LogitsArgs a)
         }
         __syncthreads();
     }
-    const float y = rep > 1.0f ? 1.0f / rep : 1.0f;
+    const Reciprocal y(rep);
     const float *bias = a.bias + (size_t)row * a.bias_cap;
     unsigned long long top = 0;
 #pragma unroll
