@@ -69,7 +69,8 @@ struct RowsArgs {
 // ---- which positions -----------------------------------------------------------
 
 // Tiles of two runs of positions, [0, s) and [lo, hi): the first ns tiles
-// cover the first, the rest the second.
+// cover the first, the rest the second (of another cache, where the first is a
+// shared prefix).
 template <int TP>
 struct RowsLine {
     int s, lo, hi, ns;
@@ -302,11 +303,18 @@ struct RowsSeen {
     const int *pos;
 };
 
+// K and V rows of the kv head: the first run's, the second's.
+template <typename KT>
+struct RowsFrom {
+    const KT *k1, *v1, *k, *v;
+    __device__ __forceinline__ RowsFrom(const KT *k0, const KT *v0) : k1(k0), v1(v0), k(k0), v(v0) {}
+    __device__ __forceinline__ RowsFrom(const KT *pk, const KT *pv, const KT *k0, const KT *v0) : k1(pk), v1(pv), k(k0), v(v0) {}
+};
+
 // Tiles u, u + step, .. below u1 of `line` into the wave's rows (loaded, not yet
-// converted), K and V rows of the kv head at kb and vb.  MASKED: rows see
-// different positions (seen).
+// converted).  MASKED: rows see different positions (seen).
 template <int DH, typename KT, int RT, bool MASKED>
-__device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb, const KT *vb,
+__device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const RowsFrom<KT> &from,
                                           const RowsLine<rw_tp<KT>()> &line0, int u, int u1, int step, const RowsSeen *seen)
 {
 #pragma clang fp contract(off)
@@ -326,7 +334,7 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
     auto load_k = [&](int t) {
         int p0, cnt;
         line.tile(t, &p0, &cnt);
-        const char *base = (const char *)uniform_ptr(kb + (size_t)p0 * DH);
+        const char *base = (const char *)uniform_ptr((t < line.ns ? from.k1 : from.k) + (size_t)p0 * DH);
 #pragma unroll
         for (int c = 0; c < C; c++) {
             const unsigned at = (unsigned)min(16 * c + col, cnt - 1) * (DH * ES);
@@ -345,7 +353,7 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const KT *kb,
     auto load_v = [&](int t) {
         int p0, cnt;
         line.tile(t, &p0, &cnt);
-        const char *base = (const char *)uniform_ptr(vb + (size_t)p0 * DH);
+        const char *base = (const char *)uniform_ptr((t < line.ns ? from.v1 : from.v) + (size_t)p0 * DH);
 #pragma unroll
         for (int r = 0; r < VR; r++) {
             const int row = 16 * (r / 4) + 4 * g + r % 4;
@@ -648,7 +656,7 @@ __device__ __forceinline__ void few_exchange(bool on, float a, float b, float &x
 
 // As rows_walk: tiles u, u + step, .. below u1.
 template <int DH>
-__device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const float *vb, const RowsLine<FEW_TP> &line0, int u,
+__device__ __forceinline__ void few_walk(RowsFew<DH> &w, const RowsFrom<float> &from, const RowsLine<FEW_TP> &line0, int u,
                                          int u1, int step)
 {
 #pragma clang fp contract(off)
@@ -660,17 +668,17 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
     const int lane = threadIdx.x & 63, b = lane >> 2, q = lane / GL;
     const float c2 = 1.44269504088896341f / sqrtf((float)DH);
     f32x4 kr[NV], vr[NV];
-    auto load = [&](const float *from, int t, f32x4 (&to)[NV]) {
+    auto load = [&](const float *run1, const float *run2, int t, f32x4 (&to)[NV]) {
         int p0, cnt;
         line.tile(t, &p0, &cnt);
-        const char *base = (const char *)uniform_ptr(from + (size_t)p0 * DH);
+        const char *base = (const char *)uniform_ptr((t < line.ns ? run1 : run2) + (size_t)p0 * DH);
 #pragma unroll
         for (int n = 0; n < NV; n++)
             to[n] = ldg((const f32x4 *)(base + ((unsigned)min(NQ * n + q, cnt - 1) * (DH * 4) + 16 * (lane % GL))));
     };
     if (u >= u1) return;
-    load(kb, u, kr);
-    load(vb, u, vr);
+    load(from.k1, from.k, u, kr);
+    load(from.v1, from.v, u, vr);
     for (;;) {
         const bool more = u + step < u1;
         int p0, cnt;
@@ -696,7 +704,7 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
 #pragma unroll
                 for (int j = 0; j < NJ; j++) s[j] = __builtin_amdgcn_mfma_f32_4x4x1f32(z[j][t], w.q[t][e], s[j], 0, 0, 0);
         }
-        if (more) load(kb, u + step, kr);
+        if (more) load(from.k1, from.k, u + step, kr);
         // ---- reduce-scatter: x[4j + i] is row NQ (4j + i) + q of the tile
         float x[NV], p[2];
 #pragma unroll
@@ -751,7 +759,7 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const float *kb, const 
         w.add(vr, p, std::make_integer_sequence<int, NV>());
         if (!more) return;
         u += step;
-        load(vb, u, vr);
+        load(from.v1, from.v, u, vr);
     }
 }
 
@@ -914,7 +922,7 @@ RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window,
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks);
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx);
 
-int launch_attn_window(const RowsArgs &a, hipStream_t s);
+int launch_attn_window(const RowsArgs &a, hipStream_t s);   // (with a.prefix: behind it, every item whole)
 int launch_attn_window_prompt(const RowsArgs &a, hipStream_t s);
 int launch_attn_shared(const RowsArgs &a, hipStream_t s);
 

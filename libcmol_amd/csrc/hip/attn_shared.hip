@@ -4,8 +4,11 @@
 // the prefix's positions together, RT tiles per work-group and the positions in
 // `parts`; the sessions' own positions are walked as single tokens are, in
 // balanced ranges.  Both kinds of work-group are one launch, and the merge
-// takes the parts and the pieces of a row.
+// takes the parts and the pieces of a row.  Where that costs more than it saves, a
+// session is one work-group's of k_window (attn_window.hip).
 #include "attn_rows.h"
+
+#include <cstdlib>
 
 constexpr int SH_NW = 4;   // waves per work-group
 
@@ -38,7 +41,8 @@ __device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH, SH
         return a.q + ((size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G) * DH;
     });
     const size_t base = (size_t)kvh * a.prefix_ctx * DH;
-    rows_walk<DH, KT, RT, false>(w, (const KT *)a.pk + base, (const KT *)a.pv + base, line, u0 + wid, u1, SH_NW, nullptr);
+    rows_walk<DH, KT, RT, false>(w, RowsFrom<KT>((const KT *)a.pk + base, (const KT *)a.pv + base), line, u0 + wid, u1, SH_NW,
+                                 nullptr);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         if (r0 + r >= rows) return;
@@ -66,9 +70,9 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, M &meet, unsigned 
     typename std::conditional<FEW, RowsFew<DH>, RowsWave<DH, KT, 1>>::type w;
     w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     const size_t base = (size_t)p.slot * a.slot_stride + (size_t)kvh * a.max_ctx * DH;
-    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
-    if constexpr (FEW) few_walk<DH>(w, k, v, line, p.u0 + wid, p.u1, SH_NW);
-    else rows_walk<DH, KT, 1, false>(w, k, v, line, p.u0 + wid, p.u1, SH_NW, nullptr);
+    const RowsFrom<KT> from((const KT *)a.k + base, (const KT *)a.v + base);
+    if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, p.u1, SH_NW);
+    else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, p.u1, SH_NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
@@ -141,9 +145,34 @@ static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt, int kv
     return (int)std::max(1L, std::min(wgs / blocks, (tiles + SH_NW - 1) / SH_NW));
 }
 
+// Whether every session is one work-group's (per kv head), prefix and own
+// positions together: no merge launch, but the prefix read by each.  By what both
+// are estimated to cost, in microseconds, from the most positions the call may
+// have: a work-group's start and end, its positions' steps and bytes (more than
+// one per CU take turns); two launches, their pieces, the prefix's products (an
+// f32 one as eight f16 ones) and the own positions' bytes.  Fitted to 2 .. 64
+// sessions of 16/4 heads of 128 and 9/3 of 64 behind 100 .. 3200 positions with up
+// to 100 .. 1500 of their own.  Both sides measured, apart and together: 8 sessions
+// of 9/3 heads, fp16, 200 + 200: 8.9 and 5.6 us, 1600 + 128: 9.3 and 12.3; 64 of
+// 16/4, fp16, 800 + 512: 22.2 and 17.2; 8 of 16/4, fp32, 200 + 200: 10.2 and 9.7,
+// 800 + 128: 9.5 and 15.4.  (CMOL_SHARED_WHOLE=0 / 1: never / always)
+static bool shared_whole(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx, int kv_f16)
+{
+    const char *e = getenv("CMOL_SHARED_WHOLE");
+    if (e && (e[0] == '0' || e[0] == '1')) return e[0] == '1';
+    const double wgs = (double)n * n_kv * ceil_div(n_heads / n_kv, 16), row = d_head * (kv_f16 ? 4.0 : 8.0);   // bytes of K and V
+    const double seen = (double)prefix + max_ctx;
+    const double together = 4.3 + 0.0019 * seen + 11e-6 * seen * row * std::max(1.0, wgs / 256);
+    const double apart = 8.9 + 0.015 * n * n_kv + 5.1e-9 * n * n_heads * prefix * d_head * (kv_f16 ? 1 : 8) +
+                         6.6e-8 * n * n_kv * max_ctx * row;
+    return together < apart;
+}
+
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
 {
     RowsPlan p;
+    if (shared_whole(n, n_heads, n_kv, d_head, prefix, max_ctx, 0) && shared_whole(n, n_heads, n_kv, d_head, prefix, max_ctx, 1))
+        return p;
     const int G = n_heads / n_kv;
     p.parts = 1;
     for (int f16 = 0; f16 < 2; f16++)
@@ -157,6 +186,10 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
 int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
+    if (shared_whole(a.n, a.n_heads, a.n_kv, a.d_head, a.prefix, a.max_ctx, a.kv_f16)) {
+        a.bal = 0;
+        return launch_attn_window(a, s);
+    }
     const int G = a.n_heads / a.n_kv, rt = shared_rt(a.n, G, a.d_head, a.kv_f16);
     a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt, a.kv_f16));
     const dim3 grid(shared_prefix_wgs(a, rt) + (unsigned)(a.n_kv * ceil_div(G, 16)) * (a.bal + a.n)), block(256);

@@ -1,5 +1,7 @@
 // attn_window.hip — attention over a sliding window with sinks (attn_rows.h):
-// single tokens of many sessions, and consecutive tokens of one.
+// single tokens of many sessions, and consecutive tokens of one.  Single tokens
+// behind a short shared prefix (attn_shared.hip) are single tokens whose first
+// run of positions is in another cache.
 #include "attn_rows.h"
 
 #include <cstdlib>
@@ -19,21 +21,32 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 2
     const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const RowsPiece p = rows_piece<TP>(a, slot);
     if (p.item < 0) return;
-    const RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
+    RowsLine<TP> line = rows_line<TP>(p.L - 1, p.L - 1, a.window, a.sinks);
+    int u1 = p.u1;
+    if (a.prefix) {
+        line.s = a.prefix;
+        line.ns = (a.prefix + TP - 1) / TP;
+        u1 = line.tiles();
+    }
+    const bool none = u1 == 0;   // (a whole item's)
     const size_t row0 = (size_t)p.item * a.n_heads + (size_t)kvh * G;
     typename std::conditional<FEW, RowsFew<DH>, RowsWave<DH, KT, 1>>::type w;
     w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     const size_t base = (p.L > 0 ? (size_t)p.slot * a.slot_stride : 0) + (size_t)kvh * a.max_ctx * DH;
-    const KT *k = (const KT *)a.k + base, *v = (const KT *)a.v + base;
-    if constexpr (FEW) few_walk<DH>(w, k, v, line, p.u0 + wid, p.u1, NW);
-    else rows_walk<DH, KT, 1, false>(w, k, v, line, p.u0 + wid, p.u1, NW, nullptr);
+    RowsFrom<KT> from((const KT *)a.k + base, (const KT *)a.v + base);
+    if (a.prefix) {
+        from.k1 = (const KT *)a.pk + (size_t)kvh * a.prefix_ctx * DH;
+        from.v1 = (const KT *)a.pv + (size_t)kvh * a.prefix_ctx * DH;
+    }
+    if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, u1, NW);
+    else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, u1, NW, nullptr);
     const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
         if (p.whole) {
-            const float f = p.L > 0 ? 1.0f / l : 0.0f;
-            for (auto &y : x) y = p.L > 0 ? y * f : 0.0f;
+            const float f = none ? 0.0f : 1.0f / l;
+            for (auto &y : x) y = none ? 0.0f : y * f;
             rows_store(a.out + (row0 + r) * DH + d, x);
         } else {
             rows_store(a.po + (part + r) * DH + d, x);
@@ -104,7 +117,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
     if (tid == 0) odd = 0;
     if (tid < 16) odd_row[tid] = 0;
     __syncthreads();
-    rows_walk<DH, KT, 1, true>(w, k, v, line, u0 + wid, u1, NW, &seen);
+    rows_walk<DH, KT, 1, true>(w, RowsFrom<KT>(k, v), line, u0 + wid, u1, NW, &seen);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         if (r >= nr) return;
@@ -276,7 +289,8 @@ int launch_attn_window(const RowsArgs &a, hipStream_t s)
     const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), a.bal + a.n);
     // eight waves for items that have more than one round of tiles for four
     // (d_head 256: four, for their registers)
-    const bool wide = !a.bal && a.d_head < 256 && span_tiles(a.max_ctx, a.window, a.sinks) > 4;
+    const bool wide =
+        !a.bal && a.d_head < 256 && span_tiles(a.max_ctx, a.window, a.sinks) + ceil_div(a.prefix, RW_PLAN_TP) > 4;
     const bool few = few_takes(a.d_head, a.n_heads / a.n_kv, a.kv_f16);
 #define LAUNCH(DH, KT, NW, FEW) hipLaunchKernelGGL((k_window<DH, KT, NW, FEW>), grid, dim3(NW * 64), 0, s, a)
 #define WIN_NW(DH, NW)                                        \

@@ -353,9 +353,16 @@ SHARED_CASES = [
 ]
 
 
+@pytest.mark.parametrize("form", [None, "0", "1"])
 @pytest.mark.parametrize("f16", [F32, F16])
 @pytest.mark.parametrize("heads,kv,dh,prefix,prefix_ctx,lens,max_ctx", SHARED_CASES, ids=str)
-def test_shared_against_64_bits(ctx, heads, kv, dh, prefix, prefix_ctx, lens, max_ctx, f16):
+def test_shared_against_64_bits(ctx, monkeypatch, heads, kv, dh, prefix, prefix_ctx, lens, max_ctx, f16, form):
+    """By the estimated form, the prefix read once for all ("0"), and every session
+    by itself ("1")."""
+    if form is None:
+        monkeypatch.delenv("CMOL_SHARED_WHOLE", raising=False)
+    else:
+        monkeypatch.setenv("CMOL_SHARED_WHOLE", form)
     c = native.Ctx(256 << 20)
     rng = np.random.default_rng(heads * dh + prefix)
     n = len(lens)
