@@ -41,7 +41,6 @@
 #include <utility>
 
 template <typename KT> constexpr int rw_tp() { return sizeof(KT) == 2 ? 32 : 16; }   // positions per tile
-constexpr int RW_PAD = 2;            // tiles that stand for the start of an item's piece
 constexpr float RW_LAZY = 2.0f;      // log2: weights stay below 2^(RW_SCALE + 2)
 constexpr float RW_SCALE = 12.0f;
 
@@ -59,9 +58,9 @@ struct RowsArgs {
     int prefix, prefix_ctx;
     // work split (rows_plan_*) and its partial results: (m, l, o[d_head]) per
     // query row and part; a weight sum is l 2^m
-    int bal;                   // balanced ranges of the items' own positions (0: one work-group per item)
+    int bal;                   // pieces of the items' own positions at most (0: one work-group per item)
     int parts;                 // parts of the prefix, or of a prompt block's positions
-    float *pm, *pl, *po;       // [n_kv][bal + n][G]
+    float *pm, *pl, *po;       // [n_kv][rows_slots][G]
     float *xm, *xl, *xo;       // [n_kv][n * G][parts]
     void *split;               // prompt over an fp32 cache: its f16 pairs (attn_wprompt.hip)
 };
@@ -122,31 +121,60 @@ __device__ __forceinline__ unsigned rows_tiles(const RowsArgs &a, int L)
     return L > 0 ? rows_line<TP>(L - 1, L - 1, a.window, a.sinks).tiles() : 0;
 }
 
-// Balanced ranges.  The items' tiles are laid end to end on one line, each
-// item preceded by RW_PAD tiles for the fixed cost of starting a piece; range
-// w holds the line's tiles [w R, w R + R).  The cut of item i in range w is a
-// piece, in slot w + i (unique: pieces are in line order), so an item's pieces
-// are consecutive slots and every work-group of `bal + n` finds its own piece,
-// if any, from the lengths alone.
-constexpr unsigned RW_RMIN = 4;   // tiles per range at least: one per wave
+// Pieces.  The items are cut into pieces of at most R tiles, each into equal ones
+// as far as they go, with R the least at which there are no more pieces than
+// `bal` work-groups; slot k holds the k-th piece in the items' order, so an item's
+// are consecutive, and every work-group finds its own, if any, from the lengths
+// alone.  (Ranges of one line of all tiles cut the items anywhere: 64 sessions of
+// 16/4 heads, windows of 2000, fp16: 64 us.)
+constexpr unsigned RW_RMIN = 4;   // tiles per piece to have, one per wave
 
-// A lane's item among the first 64, and the range length (every wave works
-// them out, with no barrier).
+__host__ __device__ inline int rows_slots(const RowsArgs &a) { return a.bal ? a.bal : a.n; }
+
+// a / b; `small`: a below 2^21, where half a unit more, times the hardware
+// reciprocal, is off by less than that half (an integer division is a chain of 25
+// instructions).
+__device__ __forceinline__ unsigned rows_div(unsigned a, unsigned b, bool small)
+{
+    return small ? (unsigned)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)b)) : a / b;
+}
+
+// A lane's item among the first 64, and the most tiles of a piece (every wave
+// works them out, with no barrier).
 template <int TP>
 struct RowsSpread {
     int L, slot;
-    unsigned T, R;
+    unsigned T, R, V;   // its tiles; the most of a piece; its pieces
+    bool small;   // T and R below 2^20
     __device__ __forceinline__ explicit RowsSpread(const RowsArgs &a)
     {
         const int lane = threadIdx.x & 63;
         item(a, lane);
-        unsigned t = lane < a.n ? T + RW_PAD : 0;
-        for (int b = 64; b < a.n; b += 64) {
-            int s;
-            if (b + lane < a.n) t += rows_tiles<TP>(a, rows_item(a, b + lane, &s)) + RW_PAD;
+        small = a.max_ctx < 1 << 23;
+        if (a.n <= 64) {
+            R = RW_RMIN;
+            V = (T + RW_RMIN - 1) / RW_RMIN;
+            if (wave_sum_u(V) > (unsigned)a.bal) {
+                // (at twice the least there are at most bal / 2 + n, and bal >= 2 n)
+                const unsigned t = wave_sum_u(T);
+                const unsigned r = max(RW_RMIN, small ? (unsigned)((float)t * __builtin_amdgcn_rcpf((float)a.bal)) + 1 : t / a.bal + 1);
+                for (unsigned k = 0; k <= 8; k++) {
+                    R = r + r * k / 8;
+                    V = pieces(T);
+                    if (wave_sum_u(V) <= (unsigned)a.bal) break;
+                }
+            }
+        } else {   // (at most bal - n, and one more an item)
+            unsigned t = T;
+            for (int b = 64; b < a.n; b += 64) {
+                int s;
+                if (b + lane < a.n) t += rows_tiles<TP>(a, rows_item(a, b + lane, &s));
+            }
+            R = max(RW_RMIN, (wave_sum_u(t) + a.bal - a.n - 1) / (a.bal - a.n));
+            V = pieces(T);
         }
-        R = max(RW_RMIN, (wave_sum_u(t) + a.bal - 1) / a.bal);
     }
+    __device__ __forceinline__ unsigned pieces(unsigned tiles) const { return rows_div(tiles + R - 1, R, small); }
     __device__ __forceinline__ void item(const RowsArgs &a, int i)
     {
         slot = -1;
@@ -159,7 +187,7 @@ struct RowsPiece {
     int item, L, slot, u0, u1;   // item below 0: no piece
     bool whole;                  // the item's only one
 };
-// The piece of work-group slot k, or item k whole where there are no ranges.
+// The piece of work-group slot k, or item k whole where there are no pieces.
 template <int TP>
 __device__ __forceinline__ RowsPiece rows_piece(const RowsArgs &a, int k)
 {
@@ -177,21 +205,22 @@ __device__ __forceinline__ RowsPiece rows_piece(const RowsArgs &a, int k)
     unsigned base = 0;
     p.item = -1;
     for (int b = 0; b < a.n; b += 64) {
-        if (b) x.item(a, b + lane);
-        const unsigned v = b + lane < a.n ? x.T + RW_PAD : 0, inc = wave_scan_u(v);
-        const unsigned at = base + inc - v + RW_PAD;   // the item's first tile on the line
-        const int w = k - (b + lane);
-        const uint64_t m = __ballot(x.T > 0 && w >= (int)(at / x.R) && w <= (int)((at + x.T - 1) / x.R));
+        if (b) {
+            x.item(a, b + lane);
+            x.V = x.pieces(x.T);
+        }
+        const unsigned v = x.V, inc = wave_scan_u(v), at = base + inc - v;
+        const uint64_t m = __ballot((unsigned)k - at < v);
         if (m) {
-            const int j = __builtin_ctzll(m), i = b + j;
-            const int n = __builtin_amdgcn_readlane(x.T, j);
-            const int r0 = (int)((unsigned)(k - i) * x.R - (unsigned)__builtin_amdgcn_readlane(at, j));
-            p.item = i;
+            const int j = __builtin_ctzll(m);
+            const unsigned n = __builtin_amdgcn_readlane(v, j), q = k - __builtin_amdgcn_readlane(at, j);
+            const unsigned T = __builtin_amdgcn_readlane(x.T, j), each = rows_div(T, n, x.small), more = T - each * n;
+            p.item = b + j;
             p.L = __builtin_amdgcn_readlane(x.L, j);
             p.slot = __builtin_amdgcn_readlane(x.slot, j);
-            p.u0 = max(r0, 0);
-            p.u1 = min(r0 + (int)x.R, n);
-            p.whole = r0 <= 0 && r0 + (int)x.R >= n;
+            p.u0 = q * each + min(q, more);
+            p.u1 = p.u0 + each + (q < more);
+            p.whole = n == 1;
             break;
         }
         base += __builtin_amdgcn_readlane(inc, 63);
@@ -209,14 +238,12 @@ __device__ __forceinline__ int rows_pieces(const RowsArgs &a, int i, int *first)
         return rows_item(a, i, &slot) > 0 ? 1 : 0;
     }
     const int lane = threadIdx.x & 63;
-    const unsigned T = rows_tiles<TP>(a, rows_item(a, i, &slot));
     const RowsSpread<TP> x(a);
-    unsigned pre = lane < min(i, 64) ? x.T + RW_PAD : 0;
+    unsigned pre = lane < min(i, 64) ? x.V : 0;
     for (int b = 64; b < i; b += 64)
-        if (b + lane < i) pre += rows_tiles<TP>(a, rows_item(a, b + lane, &slot)) + RW_PAD;
-    const unsigned at = wave_sum_u(pre) + RW_PAD;
-    *first = (int)(at / x.R) + i;
-    return T ? (int)((at + T - 1) / x.R - at / x.R) + 1 : 0;
+        if (b + lane < i) pre += x.pieces(rows_tiles<TP>(a, rows_item(a, b + lane, &slot)));
+    *first = wave_sum_u(pre);
+    return i < 64 ? __builtin_amdgcn_readlane(x.V, i) : x.pieces(rows_tiles<TP>(a, rows_item(a, i, &slot)));
 }
 
 // ---- the walk ------------------------------------------------------------------
@@ -905,11 +932,21 @@ constexpr int RW_WGS = 512;   // work-groups of a call to aim for: two per CU
 
 inline int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
-// Balanced ranges for n items of up to `span` tiles on `heads` work-groups
-// each, 0 (an item whole) where the items alone fill the chip or an item has at
-// most `whole` tiles.  (Tiles of 32 positions: a plan serves both cache types.)
-constexpr int RW_PLAN_TP = 32;
-int rows_plan_bal(int n, long heads, long span, long whole);
+constexpr int RW_PLAN_TP = 32;   // (a plan serves both cache types)
+
+// Microseconds of a call whose items, of up to `seen` positions, are one
+// work-group of eight waves each (`wgs` of them): its start and end, its
+// positions' steps and bytes (more than one per CU take turns).
+inline double rows_together(double wgs, double seen, int d_head, int kv_f16)
+{
+    return 4.3 + 0.0019 * seen + 11e-6 * seen * d_head * (kv_f16 ? 4 : 8) * std::max(1.0, wgs / 256);
+}
+// CMOL_SESSION_WHOLE=0 / 1: items in pieces / whole wherever there is a choice
+// (-1: by what both are estimated to cost).
+int rows_whole_env();
+// Pieces for n items of up to `span` tiles on `heads` work-groups each, 0 where
+// the items alone fill the chip.
+int rows_plan_bal(int n, long heads, long span);
 
 // What a call of these shapes splits into, and the number of its partial
 // results.
@@ -918,7 +955,7 @@ struct RowsPlan {
     size_t pieces = 0, cross = 0;   // pm / pl / po, and xm / xl / xo
     size_t split = 0;               // bytes of the f16 pairs
 };
-RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks);
+RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks);
 RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks);
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx);
 

@@ -3,12 +3,10 @@
 // sessions' query rows (n G of them, session-major) form tiles of 16 that walk
 // the prefix's positions together, RT tiles per work-group and the positions in
 // `parts`; the sessions' own positions are walked as single tokens are, in
-// balanced ranges.  Both kinds of work-group are one launch, and the merge
-// takes the parts and the pieces of a row.  Where that costs more than it saves, a
-// session is one work-group's of k_window (attn_window.hip).
+// pieces.  Both kinds of work-group are one launch, and the merge takes the
+// parts and the pieces of a row.  Where that costs more than it saves, a session
+// is one work-group's of k_window (attn_window.hip).
 #include "attn_rows.h"
-
-#include <cstdlib>
 
 constexpr int SH_NW = 4;   // waves per work-group
 
@@ -73,7 +71,7 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, M &meet, unsigned 
     const RowsFrom<KT> from((const KT *)a.k + base, (const KT *)a.v + base);
     if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, p.u1, SH_NW);
     else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, p.u1, SH_NW, nullptr);
-    const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
+    const size_t part = ((size_t)kvh * rows_slots(a) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
@@ -109,7 +107,7 @@ __global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
     int first;
     const int np = rows_pieces<TP>(a, i, &first);
     const size_t x0 = ((size_t)kvh * a.n * G + (size_t)i * G + h % G) * a.parts;
-    const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
+    const size_t p0 = ((size_t)kvh * rows_slots(a) + first) * G + h % G;
     const f32x4 o = rows_sum<DH, 256 / LPR>(
         pre + np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
             const bool own = j >= pre;
@@ -148,24 +146,21 @@ static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt, int kv
 // Whether every session is one work-group's (per kv head), prefix and own
 // positions together: no merge launch, but the prefix read by each.  By what both
 // are estimated to cost, in microseconds, from the most positions the call may
-// have: a work-group's start and end, its positions' steps and bytes (more than
-// one per CU take turns); two launches, their pieces, the prefix's products (an
-// f32 one as eight f16 ones) and the own positions' bytes.  Fitted to 2 .. 64
-// sessions of 16/4 heads of 128 and 9/3 of 64 behind 100 .. 3200 positions with up
-// to 100 .. 1500 of their own.  Both sides measured, apart and together: 8 sessions
-// of 9/3 heads, fp16, 200 + 200: 8.9 and 5.6 us, 1600 + 128: 9.3 and 12.3; 64 of
-// 16/4, fp16, 800 + 512: 22.2 and 17.2; 8 of 16/4, fp32, 200 + 200: 10.2 and 9.7,
-// 800 + 128: 9.5 and 15.4.  (CMOL_SHARED_WHOLE=0 / 1: never / always)
+// have; apart: two launches, their pieces, the prefix's products (an f32 one as
+// eight f16 ones) and the own positions' bytes.  Fitted to 2 .. 64 sessions of 16/4
+// heads of 128 and 9/3 of 64 behind 100 .. 3200 positions with up to 100 .. 1500 of
+// their own.  Both sides measured, apart and together: 8 sessions of 9/3 heads,
+// fp16, 200 + 200: 8.9 and 5.6 us, 1600 + 128: 9.3 and 12.3; 64 of 16/4, fp16,
+// 800 + 512: 22.2 and 17.2; 8 of 16/4, fp32, 200 + 200: 10.2 and 9.7, 800 + 128: 9.5
+// and 15.4.
 static bool shared_whole(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx, int kv_f16)
 {
-    const char *e = getenv("CMOL_SHARED_WHOLE");
-    if (e && (e[0] == '0' || e[0] == '1')) return e[0] == '1';
-    const double wgs = (double)n * n_kv * ceil_div(n_heads / n_kv, 16), row = d_head * (kv_f16 ? 4.0 : 8.0);   // bytes of K and V
-    const double seen = (double)prefix + max_ctx;
-    const double together = 4.3 + 0.0019 * seen + 11e-6 * seen * row * std::max(1.0, wgs / 256);
+    const int e = rows_whole_env();
+    if (e >= 0) return e;
+    const double wgs = (double)n * n_kv * ceil_div(n_heads / n_kv, 16);
     const double apart = 8.9 + 0.015 * n * n_kv + 5.1e-9 * n * n_heads * prefix * d_head * (kv_f16 ? 1 : 8) +
-                         6.6e-8 * n * n_kv * max_ctx * row;
-    return together < apart;
+                         6.6e-8 * n * n_kv * max_ctx * d_head * (kv_f16 ? 4 : 8);
+    return rows_together(wgs, (double)prefix + max_ctx, d_head, kv_f16) < apart;
 }
 
 RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, int max_ctx)
@@ -178,8 +173,9 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
     for (int f16 = 0; f16 < 2; f16++)
         p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16), f16));
     p.cross = prefix ? (size_t)n * n_heads * p.parts : 0;
-    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP), 8);
-    p.pieces = (size_t)n_kv * (p.bal + n) * G;
+    // (own contexts of two tiles a wave at most: not cut)
+    if (max_ctx > 8 * RW_PLAN_TP) p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP));
+    p.pieces = (size_t)n_kv * (p.bal ? p.bal : n) * G;
     return p;
 }
 
@@ -192,7 +188,7 @@ int launch_attn_shared(const RowsArgs &a0, hipStream_t s)
     }
     const int G = a.n_heads / a.n_kv, rt = shared_rt(a.n, G, a.d_head, a.kv_f16);
     a.parts = std::min(a.parts, shared_parts(a.n, a.n_heads, a.n_kv, a.prefix, rt, a.kv_f16));
-    const dim3 grid(shared_prefix_wgs(a, rt) + (unsigned)(a.n_kv * ceil_div(G, 16)) * (a.bal + a.n)), block(256);
+    const dim3 grid(shared_prefix_wgs(a, rt) + (unsigned)(a.n_kv * ceil_div(G, 16)) * rows_slots(a)), block(256);
     const bool few = few_takes(a.d_head, G, a.kv_f16);
 #define SHA(DH)                                                                                                  \
     if constexpr (few_takes(DH, 1, 0))                                                                           \

@@ -9,7 +9,7 @@
 // ---- single tokens ---------------------------------------------------------------
 
 // Work-group of NW waves (16 query heads of a kv head, slot): the piece of that
-// slot, or item `slot` whole where there are no balanced ranges.
+// slot, or item `slot` whole where there are no pieces.
 template <int DH, typename KT, int NW, bool FEW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window(RowsArgs a)
 {
@@ -40,7 +40,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 2
     }
     if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, u1, NW);
     else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, u1, NW, nullptr);
-    const size_t part = ((size_t)kvh * (a.bal + a.n) + slot) * G;
+    const size_t part = ((size_t)kvh * rows_slots(a) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
         if (r >= G) return;
@@ -69,7 +69,7 @@ __global__ __launch_bounds__(256) void k_window_merge(RowsArgs a)
     int first;
     const int np = rows_pieces<TP>(a, i, &first);
     if (np == 1) return;   // finished by its only piece
-    const size_t p0 = ((size_t)kvh * (a.bal + a.n) + first) * G + h % G;
+    const size_t p0 = ((size_t)kvh * rows_slots(a) + first) * G + h % G;
     const f32x4 o = rows_sum<DH, 256 / LPR>(np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
         const size_t at = p0 + (size_t)j * G;
         *m = a.pm + at;
@@ -203,25 +203,45 @@ static long span_tiles(int max_ctx, int window, int sinks)
     return std::min((long)ceil_div(w, RW_PLAN_TP) + ceil_div(s, RW_PLAN_TP), (long)ceil_div(max_ctx, RW_PLAN_TP) + 2);
 }
 
-int rows_plan_bal(int n, long heads, long span, long whole)
+int rows_whole_env()
 {
-    if (span <= whole || n * heads >= RW_WGS || n * (span + RW_PAD) > INT32_MAX / 4) return 0;
-    // (two ranges an item at least: with fewer the longest piece is twice the mean.
-    // 64 sessions of 4 kv heads, windows of 2048 over fp16: 51.1 us with one, 47.9)
-    const long want = std::max(RW_WGS / heads - n, 2L * n);
-    return (int)std::min(want, n * (long)ceil_div(span + RW_PAD, RW_RMIN));
+    const char *e = getenv("CMOL_SESSION_WHOLE");
+    return e && (e[0] == '0' || e[0] == '1') ? e[0] - '0' : -1;
 }
 
-// An item of up to this many tiles is one work-group's, of eight waves: the
-// waves' rounds cost less than a merge launch.
-constexpr int WIN_WHOLE = 32;
+int rows_plan_bal(int n, long heads, long span)
+{
+    if (n * heads >= RW_WGS || n * span > INT32_MAX / 4) return 0;
+    return (int)std::max(std::min(RW_WGS / heads, n * (long)ceil_div(span, RW_RMIN)), 2L * n);
+}
 
-RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int max_ctx, int window, int sinks)
+// Whether every item is one work-group's: no merge launch and no search, but the
+// longest item is the call's time.  By what both are estimated to cost at most,
+// the pieces' bytes at six tenths of what they may be, and up to WIN_RISK
+// microseconds (a batch whose sessions are short but for one costs as much, where
+// pieces would take 9).  Fitted to 1 .. 64 sessions of 16/4 heads of 128 and 9/3 of
+// 64, windows of 300 .. 4000; both sides measured, in pieces and whole: one session
+// of 16/4, fp32, window 900: 8.8 and 15.6 us, of 9/3, fp16: 8.5 and 8.0; 16 of 9/3, fp32,
+// 1400: 13.6 and 12.9; 64 of 9/3, fp16, 2000: 24.2 and 18.0.
+constexpr double WIN_RISK = 16;
+static bool window_whole(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks, int kv_f16)
+{
+    const int e = rows_whole_env();
+    if (e >= 0) return e;
+    const double heads = (double)n_kv * ceil_div(n_heads / n_kv, 16), row = d_head * (kv_f16 ? 4 : 8);
+    const double seen = std::min((double)max_ctx, (double)std::min(window, max_ctx) + std::min(sinks, max_ctx));
+    const double together = rows_together(n * heads, seen, d_head, kv_f16);
+    return together < WIN_RISK && together < 8 + 0.008 * n * n_kv + 0.6 * n * heads * seen * row / 5.6e6;
+}
+
+RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int d_head, int max_ctx, int window, int sinks)
 {
     RowsPlan p;
     const int G = n_heads / n_kv;
-    p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks), WIN_WHOLE);
-    if (p.bal) p.pieces = (size_t)n_kv * (p.bal + n) * G;
+    if (!window_whole(n, n_heads, n_kv, d_head, max_ctx, window, sinks, 0) ||
+        !window_whole(n, n_heads, n_kv, d_head, max_ctx, window, sinks, 1))
+        p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks));
+    if (p.bal) p.pieces = (size_t)n_kv * p.bal * G;
     return p;
 }
 
@@ -284,9 +304,11 @@ RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx,
     return p;
 }
 
-int launch_attn_window(const RowsArgs &a, hipStream_t s)
+int launch_attn_window(const RowsArgs &a0, hipStream_t s)
 {
-    const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), a.bal + a.n);
+    RowsArgs a = a0;
+    if (a.prefix || window_whole(a.n, a.n_heads, a.n_kv, a.d_head, a.max_ctx, a.window, a.sinks, a.kv_f16)) a.bal = 0;
+    const dim3 grid(a.n_kv * ceil_div(a.n_heads / a.n_kv, 16), rows_slots(a));
     // eight waves for items that have more than one round of tiles for four
     // (d_head 256: four, for their registers)
     const bool wide =

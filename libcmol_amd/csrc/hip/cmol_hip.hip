@@ -622,7 +622,7 @@ size_t window_bytes(bool prompt, int n, int n_heads, int n_kv, int d_head, int m
         return 0;
     }
     *p = prompt ? rows_plan_prompt(n, n_heads, n_kv, d_head, max_ctx, window, sinks)
-                : rows_plan_window(n, n_heads, n_kv, max_ctx, window, sinks);
+                : rows_plan_window(n, n_heads, n_kv, d_head, max_ctx, window, sinks);
     return plan_bytes(*p, d_head);
 }
 

@@ -120,11 +120,21 @@ WINDOW_CASES = [
 ]
 
 
+def session_form(monkeypatch, form):
+    """Sessions in pieces ("0"), whole ("1"), or (None) as estimated."""
+    if form is None:
+        monkeypatch.delenv("CMOL_SESSION_WHOLE", raising=False)
+    else:
+        monkeypatch.setenv("CMOL_SESSION_WHOLE", form)
+
+
+@pytest.mark.parametrize("form", [None, "0", "1"])
 @pytest.mark.parametrize("f16", [F32, F16])
 @pytest.mark.parametrize("heads,kv,dh,max_ctx,lens,window,sinks", WINDOW_CASES, ids=str)
-def test_window_against_64_bits(ctx, heads, kv, dh, max_ctx, lens, window, sinks, f16):
+def test_window_against_64_bits(ctx, monkeypatch, heads, kv, dh, max_ctx, lens, window, sinks, f16, form):
     """Every position that no row sees holds NaN or an infinity; queries of
     half of the rows are large, so their softmaxes are peaked."""
+    session_form(monkeypatch, form)
     c = native.Ctx(256 << 20)
     rng = np.random.default_rng(heads * dh + len(lens))
     n = len(lens)
@@ -359,10 +369,7 @@ SHARED_CASES = [
 def test_shared_against_64_bits(ctx, monkeypatch, heads, kv, dh, prefix, prefix_ctx, lens, max_ctx, f16, form):
     """By the estimated form, the prefix read once for all ("0"), and every session
     by itself ("1")."""
-    if form is None:
-        monkeypatch.delenv("CMOL_SHARED_WHOLE", raising=False)
-    else:
-        monkeypatch.setenv("CMOL_SHARED_WHOLE", form)
+    session_form(monkeypatch, form)
     c = native.Ctx(256 << 20)
     rng = np.random.default_rng(heads * dh + prefix)
     n = len(lens)
