@@ -85,6 +85,11 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, M &meet, unsigned 
     else rows_finish(w, meet, put);
 }
 
+// 48 sessions of 16/4 heads of 128 behind 2000 positions, fp32: 18.5 us, of which
+// the prefix's f32 products are 6 at least; 32 sessions behind 8192, fp16, 56 MB:
+// 19.3 us, most of it the start, the search for a piece and the end of work-groups
+// with few steps.  The prefix's rows (columns of a product) are all used: n G of
+// them share a tile of 16.
 template <int DH, typename KT, int RT, bool FEW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_shared(RowsArgs a)
 {
@@ -98,6 +103,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
     else shared_own<DH, KT, false>(a, meet.rows, blockIdx.x - pre);
 }
 
+// One work-group per (query head, session): the prefix's parts and the session's
+// pieces, 4.4 .. 5.3 us.
 template <int DH, int TP>
 __global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
 {

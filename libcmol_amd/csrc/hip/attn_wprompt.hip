@@ -23,9 +23,13 @@
 //     then follows what reaches the output, and the weights' sum takes it out.
 // Products are exact (lo.lo, below 2^-22 of each, is left out over fp32), sums
 // fp32; the query is split as the walk's of attn_rows.h, the weights too.
-// A tile has 2 x 2 (fp32 3) products per (row tile, 16 positions, 32
-// dimensions): bound by the matrix pipe and by the softmax's vector
-// instructions beside it.
+// Of the four pairs of halves a product over fp16 has two (the cache's is one
+// number), over fp32 three.  Bound by the matrix pipe and by the softmax's vector
+// instructions beside it: 4096 tokens of 16/4 heads of 128, window 2048, fp32 (155
+// GFLOP in products): 162 us, 0.95 PFLOP/s, where a large library product reaches
+// 1.15; 700 tokens behind 5000, fp16 (24 GFLOP), 41.5 us, a start and an end of
+// about 8 among them.  Why 128 rows: a tile read from LDS serves two row tiles a
+// wave; 256 would leave short prompts too few work-groups.
 #include "attn_rows.h"
 #include "lds_limit.h"
 
@@ -54,6 +58,9 @@ constexpr int WP_FAR = 90;                       // most that V's exponents may 
 template <int DH>
 constexpr int wp_tile_halves() { return WP_TP * DH * 4; }
 
+// Bound by its bytes (4096 positions of 4 kv heads of 128: 17 MB read, 34 with the
+// pairs written and their maxima: 13 us); a work-group per tile and kv head, the
+// rows read twice, once whole for the largest of each, once in operand order.
 template <int DH>
 __global__ __launch_bounds__(256) void k_prompt_split(RowsArgs a, _Float16 *dst, int *exps, int tiles)
 {
