@@ -360,6 +360,8 @@ SHARED_CASES = [
     (16, 4, 128, 100, 128, [900, 0, 31, 899], 900), (4, 2, 256, 70, 70, [600, 3, 0], 600),
     # a long prefix before a few rows: many parts
     (4, 1, 64, 9000, 9000, [3, 0], 16), (2, 1, 16, 20000, 20000, [40], 64),
+    # two row tiles a work-group at the smallest d_head
+    (16, 2, 16, 200, 200, [30, 5, 0, 64], 64),
 ]
 
 
@@ -704,6 +706,59 @@ def test_captured_steps(ctx):
         rt.hipGraphExecDestroy(ex)
         rt.hipGraphDestroy(graph)
     other.close()
+
+
+@pytest.mark.parametrize("form", ["0", "1"])
+@pytest.mark.parametrize("f16", [F32, F16])
+def test_captured_prompts(ctx, monkeypatch, f16, form):
+    """A prompt in both of its forms captured into a graph and replayed over
+    other queries and another cache in the same places, with an eager prompt
+    between; its result is the eager call's, bit for bit."""
+    prompt_form(monkeypatch, form)
+    rt, L = hiprt.rt(), native.lib()
+    stream = C.c_void_p(L.cmolhip_stream(ctx.h))
+    heads, kv, dh, n, pos0, max_ctx, window, sinks = 16, 4, 128, 70, 300, 400, 150, 4
+    rng = np.random.default_rng(12)
+    need = L.cmolhip_attn_window_prompt_bytes(n, heads, kv, dh, max_ctx, window, sinks)
+    size = kv * max_ctx * dh * (2 if f16 else 4)
+    ws, out, dq, dk, dv = ctx.alloc(need), ctx.alloc(n * heads * dh * 4), ctx.alloc(n * heads * dh * 4), ctx.alloc(size), ctx.alloc(size)
+    graph, ex = C.c_void_p(), C.c_void_p()
+    assert rt.hipStreamBeginCapture(stream, 1) == 0   # thread-local mode
+    native.check(L.cmolhip_attn_window_prompt(ctx.h, n, pos0, p(dq), p(dk), p(dv), heads, kv, dh, max_ctx, f16, window, sinks,
+                                              p(ws), need, p(out)))
+    assert rt.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert rt.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+    for turn in range(3):
+        q = rng.standard_normal((n, heads, dh)).astype(np.float32)
+        k, v = (rand_cache(rng, (kv, max_ctx, dh), f16) for _ in range(2))
+        for d, x in ((dq, q), (dk, k), (dv, v), (out, np.full(n * heads * dh, 777.0, np.float32))):
+            ctx.h2d(d, x)
+        assert rt.hipGraphLaunch(ex, stream) == 0
+        native.check(L.cmolhip_synchronize(ctx.h))
+        got = ctx.d2h(out, (n, heads, dh), np.float32)
+        eager = prompt_call(ctx, q, ctx.upload(k), ctx.upload(v), pos0, heads, kv, dh, max_ctx, f16, window, sinks)
+        assert np.array_equal(got, eager), f"replay {turn}"
+        want, tol = reference(q[-1].astype(np.float64), k.astype(np.float64), v.astype(np.float64),
+                              window_seen(pos0 + n, max_ctx, window, sinks))
+        close(got[-1], want, tol, f"replay {turn}")
+    rt.hipGraphExecDestroy(ex)
+    rt.hipGraphDestroy(graph)
+
+
+def test_equal_calls_give_equal_bits(ctx):
+    """The same call twice, its scratch full of something else: no order of work
+    reaches the result."""
+    heads, kv, dh, max_ctx = 8, 2, 128, 1500
+    rng = np.random.default_rng(13)
+    for f16 in (F32, F16):
+        q = rng.standard_normal((5, heads, dh)).astype(np.float32)
+        k, v = (rand_cache(rng, (5, kv, max_ctx, dh), f16) for _ in range(2))
+        dk, dv = ctx.upload(k), ctx.upload(v)
+        lens = [1500, 3, 700, 0, 64]
+        a = [window_call(ctx, q, dk, dv, None, 0, lens, heads, kv, dh, max_ctx, f16, 1300, 4) for _ in range(2)]
+        assert np.array_equal(*a)
+        a = [shared_call(ctx, q, dk, dv, 1200, max_ctx, dk, dv, None, 0, lens, heads, kv, dh, max_ctx, f16) for _ in range(2)]
+        assert np.array_equal(*a)
 
 
 def test_steps_of_two_threads(ctx):
