@@ -866,13 +866,12 @@ __device__ void row_walk(RowState<DH> &r, const KT *k, const KT *v, int t0, int 
 // ---- partial results -------------------------------------------------------------
 
 // The sum of a row's partial results by the LPR SG threads (d4, sg) of it, SG
-// groups taking every SG-th; at(j): where the j-th of np is.  Group 0's
-// threads get the finished dimensions 4 d4 .. +3 (np 0: zeros).
-template <int DH, int SG, typename F>
+// groups taking every SG-th, U at a time; at(j): where the j-th of np is.  Group
+// 0's threads get the finished dimensions 4 d4 .. +3 (np 0: zeros).
+template <int DH, int SG, int U, typename F>
 __device__ __forceinline__ f32x4 rows_sum(int np, int d4, int sg, F at)
 {
 #pragma clang fp contract(off)
-    constexpr int U = 4;
     float mx = -INFINITY, L = 0.0f;
     f32x4 acc = {};
     for (int j0 = sg; j0 < np; j0 += U * SG) {
@@ -880,6 +879,8 @@ __device__ __forceinline__ f32x4 rows_sum(int np, int d4, int sg, F at)
         f32x4 po[U];
 #pragma unroll
         for (int i = 0; i < U; i++) {
+            pm[i] = -INFINITY;
+            if (SG == 1 && j0 + i >= np) continue;   // (uniform)
             const float *m, *l, *o;
             at(min(j0 + i * SG, np - 1), &m, &l, &o);
             pm[i] = j0 + i * SG < np ? *m : -INFINITY;

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void k_shared_merge(RowsArgs a)
     const int np = rows_pieces<TP>(a, i, &first);
     const size_t x0 = ((size_t)kvh * a.n * G + (size_t)i * G + h % G) * a.parts;
     const size_t p0 = ((size_t)kvh * rows_slots(a) + first) * G + h % G;
-    const f32x4 o = rows_sum<DH, 256 / LPR>(
+    const f32x4 o = rows_sum<DH, 256 / LPR, 4>(
         pre + np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
             const bool own = j >= pre;
             const size_t at = own ? p0 + (size_t)(j - pre) * G : x0 + j;

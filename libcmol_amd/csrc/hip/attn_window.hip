@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void k_window_merge(RowsArgs a)
     const int np = rows_pieces<TP>(a, i, &first);
     if (np == 1) return;   // finished by its only piece
     const size_t p0 = ((size_t)kvh * rows_slots(a) + first) * G + h % G;
-    const f32x4 o = rows_sum<DH, 256 / LPR>(np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
+    const f32x4 o = rows_sum<DH, 256 / LPR, 4>(np, tid % LPR, tid / LPR, [&](int j, const float **m, const float **l, const float **x) {
         const size_t at = p0 + (size_t)j * G;
         *m = a.pm + at;
         *l = a.pl + at;
@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void k_prompt_parts(RowsArgs a)
     if (row >= (size_t)a.n * a.n_heads) return;
     const int G = a.n_heads / a.n_kv, t = (int)(row / a.n_heads), h = (int)(row % a.n_heads), d4 = threadIdx.x % LPR;
     const size_t x0 = ((size_t)(h / G) * a.n * G + (size_t)t * G + h % G) * a.parts;
-    const f32x4 o = rows_sum<DH, 1>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
+    const f32x4 o = rows_sum<DH, 1, 8>(a.parts, d4, 0, [&](int j, const float **m, const float **l, const float **x) {
         *m = a.xm + x0 + j;
         *l = a.xl + x0 + j;
         *x = a.xo + (x0 + j) * DH;

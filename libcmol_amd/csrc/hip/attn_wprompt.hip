@@ -26,8 +26,8 @@
 // Of the four pairs of halves a product over fp16 has two (the cache's is one
 // number), over fp32 three.  Bound by the matrix pipe and by the softmax's vector
 // instructions beside it: 4096 tokens of 16/4 heads of 128, window 2048, fp32 (155
-// GFLOP in products): 162 us, 0.95 PFLOP/s, where a large library product reaches
-// 1.15; 700 tokens behind 5000, fp16 (24 GFLOP), 41.5 us, a start and an end of
+// GFLOP in products): 158 us, 0.98 PFLOP/s, where a large library product reaches
+// 1.15; 700 tokens behind 5000, fp16 (24 GFLOP), 40.4 us, a start and an end of
 // about 8 among them.  Why 128 rows: a tile read from LDS serves two row tiles a
 // wave; 256 would leave short prompts too few work-groups.
 #include "attn_rows.h"
@@ -513,6 +513,11 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
         };
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) ls[rt] = 0.0f;
+        // A wave with products ahead goes first: the other wave of its SIMD, at its
+        // barrier, masks and reference, has the vector pipe while the matrix pipe is
+        // fed (4096 tokens over fp32: 171 us without, 162 with the second product's
+        // alone, 158; 700 over fp16: 41.7, 41.2, 40.4).
+        __builtin_amdgcn_s_setprio(1);
         read_k(st ^ 1, 0, kr[0][0]);
         read_k(st ^ 1, KS, kr[0][1]);
         __builtin_amdgcn_sched_barrier(0);
@@ -530,10 +535,6 @@ void k_prompt_rows(RowsArgs a, const _Float16 *split, const int *exps, int tiles
         }
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) l[rt] = F16 ? l[rt] + ls[rt] : fmaf(ls[rt], lk, l[rt]) + lw[rt];
-        // (a wave with only products ahead goes first, so that the other wave of its
-        // SIMD has the vector pipe while the matrix pipe is fed: 32 heads, 512 tokens,
-        // fp32 at d_head 128 176 -> 170 us, fp16 128 tokens 41.9 -> 41.4)
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int d = 0; d < DT; d += 2) {
 #pragma unroll
