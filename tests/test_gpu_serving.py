@@ -787,6 +787,39 @@ def test_steps_of_two_threads(ctx):
     other.close()
 
 
+@pytest.mark.parametrize("form", [None, "0", "1"])
+@pytest.mark.parametrize("f16", [F32, F16])
+def test_as_many_rows_as_a_call_takes(ctx, monkeypatch, f16, form):
+    """65535 sessions, tokens and rows of logits."""
+    session_form(monkeypatch, form)
+    prompt_form(monkeypatch, form)
+    c = native.Ctx(512 << 20)
+    n, heads, kv, dh, max_ctx, prefix = 65535, 2, 1, 64, 3, 2
+    rng = np.random.default_rng(14)
+    q = rng.standard_normal((n, heads, dh)).astype(np.float32)
+    k, v = (rand_cache(rng, (100, kv, max_ctx, dh), f16) for _ in range(2))
+    slots, lens = rng.integers(-1, 100, n).astype(np.int32), rng.integers(-1, max_ctx + 2, n).astype(np.int32)
+    dk, dv = c.upload(k), c.upload(v)
+    win = window_call(c, q, dk, dv, slots, 0, lens, heads, kv, dh, max_ctx, f16, 2, 0)
+    sha = shared_call(c, q, dk, dv, prefix, max_ctx, dk, dv, slots, 0, lens, heads, kv, dh, max_ctx, f16)
+    long_k, long_v = (rand_cache(rng, (kv, n, dh), f16) for _ in range(2))
+    pro = prompt_call(c, q, c.upload(long_k), c.upload(long_v), 0, heads, kv, dh, n, f16, 40, 1)
+    k64, v64 = k.astype(np.float64), v.astype(np.float64)
+    for i in [0, 1, n - 2, n - 1] + [int(t) for t in rng.integers(0, n, 60)]:
+        m = 0 if slots[i] < 0 else max(0, min(lens[i], max_ctx))
+        qi = q[i].astype(np.float64)
+        close(win[i], *reference(qi, k64[slots[i]], v64[slots[i]], window_seen(m, max_ctx, 2, 0)), f"session {i}")
+        kk, vv = (np.concatenate([x[0][:, :prefix], x[slots[i]][:, :m]], 1) for x in (k64, v64))
+        close(sha[i], *reference(qi, kk, vv, np.ones(prefix + m, bool)), f"session {i} behind the prefix")
+        t = np.unique(np.concatenate([[0], np.arange(max(0, i - 39), i + 1)]))
+        close(pro[i], *reference(qi, long_k[:, t].astype(np.float64), long_v[:, t].astype(np.float64), np.ones(len(t), bool)),
+              f"token {i}")
+    c.close()
+    x = rng.standard_normal((n, 40)).astype(np.float32)
+    got, nxt = logits_call(ctx, x)
+    assert np.array_equal(got, x) and np.array_equal(nxt, x.argmax(1))
+
+
 @pytest.mark.parametrize("f16", [F32, F16])
 def test_offsets_past_32_bits(gpu, f16):
     """A cache whose positions lie more than 4 GiB from its start; only the
