@@ -167,7 +167,10 @@ __global__ __launch_bounds__(NT) void k_logits(LogitsArgs a)
         for (int e = 0; e < 4; e++)
             if (!((mw[q] >> e) & 1)) x[q][e] = -INFINITY;
         if (po) {
-            if (wide && i + 4 <= nv) *(f32x4 *)(po + i) = x[q];
+            // (a large output does not stay in the L2s, whose write-back the next kernel
+            // would wait for: 32 rows of 128256 16.3 us, 15.0 streamed)
+            if (wide && i + 4 <= nv && SLAB > 2048) __builtin_nontemporal_store(x[q], (f32x4 *)(po + i));
+            else if (wide && i + 4 <= nv) *(f32x4 *)(po + i) = x[q];
             else
 #pragma unroll
                 for (int e = 0; e < 4; e++)
