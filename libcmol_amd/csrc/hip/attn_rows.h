@@ -338,9 +338,18 @@ struct RowsFrom {
     __device__ __forceinline__ RowsFrom(const KT *pk, const KT *pv, const KT *k0, const KT *v0) : k1(pk), v1(pv), k(k0), v(v0) {}
 };
 
+// A 16-byte load; NT: of what the call reads once.
+template <bool NT, typename T>
+__device__ __forceinline__ T rows_ldg(const T *p)
+{
+    static_assert(sizeof(T) == 16, "16 bytes");
+    if constexpr (NT) return __builtin_nontemporal_load(gptr(p));
+    else return ldg(p);
+}
+
 // Tiles u, u + step, .. below u1 of `line` into the wave's rows (loaded, not yet
 // converted).  MASKED: rows see different positions (seen).
-template <int DH, typename KT, int RT, bool MASKED>
+template <int DH, typename KT, int RT, bool MASKED, bool NT>
 __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const RowsFrom<KT> &from,
                                           const RowsLine<rw_tp<KT>()> &line0, int u, int u1, int step, const RowsSeen *seen)
 {
@@ -368,12 +377,12 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const RowsFro
             if constexpr (F16) {
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    kh[c][s] = ldg((const f16x8 *)(base + (at + (64 * s + 16 * g) % (DH * ES))));
+                    kh[c][s] = rows_ldg<NT>((const f16x8 *)(base + (at + (64 * s + 16 * g) % (DH * ES))));
                     if (DH < 32 && g >= 2) kh[c][s] = f16x8{};
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < VD; i++) kf[i] = ldg((const f32x4 *)(base + (at + 64 * i + 16 * g)));
+                for (int i = 0; i < VD; i++) kf[i] = rows_ldg<NT>((const f32x4 *)(base + (at + 64 * i + 16 * g)));
             }
         }
     };
@@ -394,7 +403,7 @@ __device__ __forceinline__ void rows_walk(RowsWave<DH, KT, RT> &w, const RowsFro
             } else {
 #pragma unroll
                 for (int b = 0; b < VB / 16; b++) {
-                    const u32x4 x = ldg((const u32x4 *)(src + 16 * b));
+                    const u32x4 x = rows_ldg<NT>((const u32x4 *)(src + 16 * b));
 #pragma unroll
                     for (int e = 0; e < 4; e++) vr[r][4 * b + e] = x[e];
                 }
@@ -682,7 +691,7 @@ __device__ __forceinline__ void few_exchange(bool on, float a, float b, float &x
 }
 
 // As rows_walk: tiles u, u + step, .. below u1.
-template <int DH>
+template <int DH, bool NT>
 __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const RowsFrom<float> &from, const RowsLine<FEW_TP> &line0, int u,
                                          int u1, int step)
 {
@@ -701,7 +710,7 @@ __device__ __forceinline__ void few_walk(RowsFew<DH> &w, const RowsFrom<float> &
         const char *base = (const char *)uniform_ptr((t < line.ns ? run1 : run2) + (size_t)p0 * DH);
 #pragma unroll
         for (int n = 0; n < NV; n++)
-            to[n] = ldg((const f32x4 *)(base + ((unsigned)min(NQ * n + q, cnt - 1) * (DH * 4) + 16 * (lane % GL))));
+            to[n] = rows_ldg<NT>((const f32x4 *)(base + ((unsigned)min(NQ * n + q, cnt - 1) * (DH * 4) + 16 * (lane % GL))));
     };
     if (u >= u1) return;
     load(from.k1, from.k, u, kr);

@@ -39,7 +39,7 @@ __device__ __forceinline__ void shared_prefix(const RowsArgs &a, RowsMeet<DH, SH
         return a.q + ((size_t)(r / G) * a.n_heads + (size_t)kvh * G + r % G) * DH;
     });
     const size_t base = (size_t)kvh * a.prefix_ctx * DH;
-    rows_walk<DH, KT, RT, false>(w, RowsFrom<KT>((const KT *)a.pk + base, (const KT *)a.pv + base), line, u0 + wid, u1, SH_NW,
+    rows_walk<DH, KT, RT, false, false>(w, RowsFrom<KT>((const KT *)a.pk + base, (const KT *)a.pv + base), line, u0 + wid, u1, SH_NW,
                                  nullptr);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
@@ -69,8 +69,8 @@ __device__ __forceinline__ void shared_own(const RowsArgs &a, M &meet, unsigned 
     w.load([&](int r) { return a.q + (row0 + min(r0 + r, G - 1)) * DH; });
     const size_t base = (size_t)p.slot * a.slot_stride + (size_t)kvh * a.max_ctx * DH;
     const RowsFrom<KT> from((const KT *)a.k + base, (const KT *)a.v + base);
-    if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, p.u1, SH_NW);
-    else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, p.u1, SH_NW, nullptr);
+    if constexpr (FEW) few_walk<DH, false>(w, from, line, p.u0 + wid, p.u1, SH_NW);
+    else rows_walk<DH, KT, 1, false, false>(w, from, line, p.u0 + wid, p.u1, SH_NW, nullptr);
     const size_t part = ((size_t)kvh * rows_slots(a) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;

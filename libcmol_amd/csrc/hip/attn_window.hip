@@ -13,7 +13,7 @@
 // where there are enough (32 sessions of 16/4 heads of 128 over fp16, windows of
 // 4096, 176 MB: 34.5 us, 5.1 TB/s), else by a launch and its dependent loads (one
 // session, a window of 128: 5.1 us).
-template <int DH, typename KT, int NW, bool FEW>
+template <int DH, typename KT, int NW, bool FEW, bool NT>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window(RowsArgs a)
 {
 #pragma clang fp contract(off)
@@ -41,8 +41,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 2
         from.k1 = (const KT *)a.pk + (size_t)kvh * a.prefix_ctx * DH;
         from.v1 = (const KT *)a.pv + (size_t)kvh * a.prefix_ctx * DH;
     }
-    if constexpr (FEW) few_walk<DH>(w, from, line, p.u0 + wid, u1, NW);
-    else rows_walk<DH, KT, 1, false>(w, from, line, p.u0 + wid, u1, NW, nullptr);
+    if constexpr (FEW) few_walk<DH, NT>(w, from, line, p.u0 + wid, u1, NW);
+    else rows_walk<DH, KT, 1, false, NT>(w, from, line, p.u0 + wid, u1, NW, nullptr);
     const size_t part = ((size_t)kvh * rows_slots(a) + slot) * G;
     auto put = [&](int r, float m, float l, int d, auto &x) {
         r += r0;
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
     if (tid == 0) odd = 0;
     if (tid < 16) odd_row[tid] = 0;
     __syncthreads();
-    rows_walk<DH, KT, 1, true>(w, RowsFrom<KT>(k, v), line, u0 + wid, u1, NW, &seen);
+    rows_walk<DH, KT, 1, true, false>(w, RowsFrom<KT>(k, v), line, u0 + wid, u1, NW, &seen);
     const size_t x0 = ((size_t)kvh * rows + r0) * a.parts + part;   // + r * parts
     rows_finish(w, meet, [&](int r, float m, float l, int d, auto &x) {
         if (r >= nr) return;
@@ -310,6 +310,17 @@ RowsPlan rows_plan_prompt(int n, int n_heads, int n_kv, int d_head, int max_ctx,
     return p;
 }
 
+// Whether the caches are streamed past the L2s: where a call may read so much that
+// nothing of a cache is there again when the next call comes.  Three sets of caches
+// in turn, plain and streamed: 32 sessions of 16/4 heads of 128, windows of 4096 (268
+// MB at most) fp32 68.7 and 60.6 us, fp16 40.0 and 39.0; windows of 2000 over fp16
+// (131 MB) 29.1 and 27.8; 1400 (92 MB) 21.5 and 26.5.
+static bool window_stream(const RowsArgs &a)
+{
+    const double seen = std::min((double)a.max_ctx, (double)a.window + a.sinks);
+    return !a.prefix && seen * a.n * a.n_kv * a.d_head * (a.kv_f16 ? 4 : 8) > 110e6;
+}
+
 int launch_attn_window(const RowsArgs &a0, hipStream_t s)
 {
     RowsArgs a = a0;
@@ -320,12 +331,17 @@ int launch_attn_window(const RowsArgs &a0, hipStream_t s)
     const bool wide =
         !a.bal && a.d_head < 256 && span_tiles(a.max_ctx, a.window, a.sinks) + ceil_div(a.prefix, RW_PLAN_TP) > 4;
     const bool few = few_takes(a.d_head, a.n_heads / a.n_kv, a.kv_f16);
-#define LAUNCH(DH, KT, NW, FEW) hipLaunchKernelGGL((k_window<DH, KT, NW, FEW>), grid, dim3(NW * 64), 0, s, a)
+    const bool nt = window_stream(a);
+#define LAUNCH(DH, KT, NW, FEW)                                                                      \
+    {                                                                                                \
+        if (DH >= 64 && nt) hipLaunchKernelGGL((k_window<DH, KT, NW, FEW, DH >= 64>), grid, dim3(NW * 64), 0, s, a); \
+        else hipLaunchKernelGGL((k_window<DH, KT, NW, FEW, false>), grid, dim3(NW * 64), 0, s, a);   \
+    }
 #define WIN_NW(DH, NW)                                        \
     if constexpr (few_takes(DH, 1, 0))                        \
-        if (few) LAUNCH(DH, float, NW, true);                 \
-    if (a.kv_f16) LAUNCH(DH, _Float16, NW, false);            \
-    else if (!few) LAUNCH(DH, float, NW, false);
+        if (few) LAUNCH(DH, float, NW, true)                  \
+    if (a.kv_f16) LAUNCH(DH, _Float16, NW, false)             \
+    else if (!few) LAUNCH(DH, float, NW, false)
 #define WIN(DH)                                               \
     if constexpr (DH < 256)                                   \
         if (wide) { WIN_NW(DH, 8) }                           \

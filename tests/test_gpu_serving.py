@@ -153,6 +153,30 @@ def test_window_against_64_bits(ctx, monkeypatch, heads, kv, dh, max_ctx, lens, 
     c.close()
 
 
+@pytest.mark.parametrize("form", [None, "0", "1"])
+@pytest.mark.parametrize("f16", [F32, F16])
+@pytest.mark.parametrize("heads,kv,dh", [(16, 4, 128), (9, 3, 64), (16, 1, 64), (16, 2, 128), (8, 2, 256)])
+def test_window_of_many_long_sessions(ctx, monkeypatch, heads, kv, dh, f16, form):
+    """More than 110 MB that a call may read (sessions share three caches, which
+    read as many bytes)."""
+    session_form(monkeypatch, form)
+    c = native.Ctx(256 << 20)
+    n, max_ctx, window, sinks = 100, 6000, 5000, 4
+    rng = np.random.default_rng(heads + dh)
+    slots = rng.integers(0, 3, n).astype(np.int32)
+    lens = rng.integers(0, 400, n).astype(np.int32)
+    lens[:4], slots[5] = [6000, 5003, 1, 2000], -1
+    assert 2 * n * (window + sinks) * kv * dh * (2 if f16 else 4) > 110e6
+    q = rng.standard_normal((n, heads, dh)).astype(np.float32)
+    k, v = (rand_cache(rng, (3, kv, max_ctx, dh), f16) for _ in range(2))
+    got = window_call(c, q, c.upload(k), c.upload(v), slots, 0, lens, heads, kv, dh, max_ctx, f16, window, sinks)
+    for i in range(n):
+        seen = window_seen(lens[i] if slots[i] >= 0 else 0, max_ctx, window, sinks)
+        want, tol = reference(q[i].astype(np.float64), k[slots[i]].astype(np.float64), v[slots[i]].astype(np.float64), seen)
+        close(got[i], want, tol, f"session {i}")
+    c.close()
+
+
 @pytest.mark.parametrize("f16", [F32, F16])
 def test_window_over_slots_of_a_pool(ctx, f16):
     """Sessions in any slot, one of them twice, padding (slot -1), caches
