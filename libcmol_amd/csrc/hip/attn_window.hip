@@ -11,7 +11,7 @@
 // Work-group of NW waves (16 query heads of a kv head, slot): the piece of that
 // slot, or item `slot` whole where there are no pieces.  Bound by the cache's bytes
 // where there are enough (32 sessions of 16/4 heads of 128 over fp16, windows of
-// 4096, 176 MB: 34.5 us, 5.1 TB/s), else by a launch and its dependent loads (one
+// 4096, 176 MB: 33.9 us, 5.2 TB/s), else by a launch and its dependent loads (one
 // session, a window of 128: 5.1 us).
 template <int DH, typename KT, int NW, bool FEW, bool NT>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(DH == 256 ? 1 : 2))) void k_window(RowsArgs a)
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(DH == 256 ?
 }
 
 // The parts of (query head, token) rows, a lane per four dimensions.  Bound by the
-// partial results: five parts of 700 tokens of 16 heads of 128, 29 MB, in 7.5 us.
+// partial results: five parts of 700 tokens of 16 heads of 128, 29 MB, in 7.0 us.
 template <int DH>
 __global__ __launch_bounds__(256) void k_prompt_parts(RowsArgs a)
 {

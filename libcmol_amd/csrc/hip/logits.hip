@@ -19,7 +19,7 @@
 // every work-group reads the row's history, so where the rows alone give each CU
 // one slabs are large (SLAB 8192 on 1024 threads), else small (2048 on 256).  One
 // row of 49152: 4.6 us and 1.5 for the pick; 32 of 128256 with every part, 33 MB:
-// 15.7 and 3.9, of which the divisions of the word repeated most are 2.8.
+// 14.3 and 3.9, of which the divisions of the word repeated most are 2.8.
 #include "logits.h"
 #include "lanes.h"
 
