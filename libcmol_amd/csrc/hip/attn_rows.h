@@ -954,9 +954,9 @@ inline double rows_together(double wgs, double seen, int d_head, int kv_f16)
 // CMOL_SESSION_WHOLE=0 / 1: items in pieces / whole wherever there is a choice
 // (-1: by what both are estimated to cost).
 int rows_whole_env();
-// Pieces for n items of up to `span` tiles on `heads` work-groups each, 0 where
-// the items alone fill the chip.
-int rows_plan_bal(int n, long heads, long span);
+// Pieces for n items of up to `span` tiles on `heads` work-groups each, to make
+// `wgs` work-groups; 0 where the items alone fill the chip.
+int rows_plan_bal(int n, long heads, long span, long wgs);
 
 // What a call of these shapes splits into, and the number of its partial
 // results.

@@ -142,11 +142,12 @@ static int shared_rt(int n, int G, int d_head, int kv_f16)
 // most of two per CU (65536 positions: 84 us at 192, 71 at 448; 16000 over fp32,
 // 48 sessions: 103, 81; 320, which gives every fourth CU a second one, lies
 // between).
+constexpr int SH_WGS = 192;
 static int shared_parts(int n, int n_heads, int n_kv, int prefix, int rt, int kv_f16)
 {
     const long blocks = (long)n_kv * ceil_div((long)n * (n_heads / n_kv), 16 * rt);
     const long tiles = ceil_div(prefix, kv_f16 ? 32 : 16);
-    const long wgs = tiles * blocks > 20L * SH_NW * 192 ? 448 : 192;
+    const long wgs = tiles * blocks > 20L * SH_NW * SH_WGS ? 448 : SH_WGS;
     return (int)std::max(1L, std::min(wgs / blocks, (tiles + SH_NW - 1) / SH_NW));
 }
 
@@ -180,8 +181,11 @@ RowsPlan rows_plan_shared(int n, int n_heads, int n_kv, int d_head, int prefix, 
     for (int f16 = 0; f16 < 2; f16++)
         p.parts = std::max(p.parts, shared_parts(n, n_heads, n_kv, prefix, shared_rt(n, G, d_head, f16), f16));
     p.cross = prefix ? (size_t)n * n_heads * p.parts : 0;
-    // (own contexts of two tiles a wave at most: not cut)
-    if (max_ctx > 8 * RW_PLAN_TP) p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP));
+    // (own contexts of two tiles a wave at most: not cut; else pieces for what the
+    // prefix leaves of two work-groups per CU: 32 sessions of 16/4 heads of 128 behind
+    // 3000 positions, fp16, 21.8 us with pieces for all of them, 19.0)
+    if (max_ctx > 8 * RW_PLAN_TP)
+        p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), ceil_div(max_ctx, RW_PLAN_TP), RW_WGS - SH_WGS);
     p.pieces = (size_t)n_kv * (p.bal ? p.bal : n) * G;
     return p;
 }

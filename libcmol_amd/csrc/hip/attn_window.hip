@@ -215,10 +215,10 @@ int rows_whole_env()
     return e && (e[0] == '0' || e[0] == '1') ? e[0] - '0' : -1;
 }
 
-int rows_plan_bal(int n, long heads, long span)
+int rows_plan_bal(int n, long heads, long span, long wgs)
 {
     if (n * heads >= RW_WGS || n * span > INT32_MAX / 4) return 0;
-    return (int)std::max(std::min(RW_WGS / heads, n * (long)ceil_div(span, RW_RMIN)), 2L * n);
+    return (int)std::max(std::min(wgs / heads, n * (long)ceil_div(span, RW_RMIN)), 2L * n);
 }
 
 // Whether every item is one work-group's: no merge launch and no search, but the
@@ -246,7 +246,7 @@ RowsPlan rows_plan_window(int n, int n_heads, int n_kv, int d_head, int max_ctx,
     const int G = n_heads / n_kv;
     if (!window_whole(n, n_heads, n_kv, d_head, max_ctx, window, sinks, 0) ||
         !window_whole(n, n_heads, n_kv, d_head, max_ctx, window, sinks, 1))
-        p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks));
+        p.bal = rows_plan_bal(n, (long)n_kv * ceil_div(G, 16), span_tiles(max_ctx, window, sinks), RW_WGS);
     if (p.bal) p.pieces = (size_t)n_kv * p.bal * G;
     return p;
 }
